@@ -291,3 +291,6 @@ def client_dropout_mult(uids, n, seed, tag, layer, p):
             and not torch._C._functorch.is_batchedtensor(uids):
         return _h().client_dropout_mult(uids, int(n), int(seed), tag, int(layer), float(p))
     return ref.client_dropout_mult(uids, n, seed, tag, layer, p)
+
+
+from .layers import client_dropout, group_norm, rope_axes  # noqa: E402,F401 — differentiable, see layers.py

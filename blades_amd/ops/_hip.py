@@ -10,7 +10,8 @@ Importing this module without the built library raises — GPU tensors never
 fall back to a PyTorch implementation.
 """
 import ctypes
-from ctypes import c_float, c_int, c_long, c_uint, c_ulonglong, c_void_p
+from ctypes import c_double, c_float, c_int, c_long, c_uint, c_ulonglong, c_void_p
+from math import ceil as _ceil
 from typing import Optional
 
 import torch
@@ -1777,3 +1778,283 @@ def ce_topk(logits, labels, ks):
     if rc != 0:
         raise ValueError(f"ce_topk rejected the call (code {rc})")
     return out
+
+
+# ---------------------------------------------------------------------------
+# layers whose result for a sample does not depend on who shares the batch: group norm (ops/csrc/groupnorm.hip),
+# client-keyed dropout without a stored mask (dropout.hip), rotary positions with several axes (rope.hip)
+_DT_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACT_CODE = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+_gn_ws = _opt_sig("blades_group_norm_ws", [c_long, c_long, c_int, c_int, c_int, c_int, c_int], c_long)
+_gn_fwd = _opt_sig("blades_group_norm_forward", [_P, _P, _P, _P, c_long, c_long, c_int, c_int, c_float, c_int, c_int, c_long,
+                                                 c_long, _P, _P, _P, _P, _P, c_int, c_int, _P], c_int)
+_gn_bwd = _opt_sig("blades_group_norm_backward", [_P, _P, _P, _P, _P, _P, _P, _P, c_long, c_long, c_int, c_int, c_int, c_int,
+                                                  c_long, c_long, _P, _P, _P, _P, _P, c_long, c_int, _P, c_int, c_int, _P],
+                   c_int)
+_client_drop = _opt_sig("blades_client_dropout", [_P, _P, _P, _P, c_long, c_int, c_long, c_long, c_long, c_int, c_int, c_int,
+                                                  c_uint, c_ulonglong, c_uint, c_float, c_int, c_int, _P], c_int)
+_rope = _opt_sig("blades_rope_axes", [_P, _P, _P, c_int, c_long, c_long, c_long, c_int, c_int, c_int, c_long, c_long, c_long,
+                                      c_long, c_int, _P, c_int, c_double, c_int, c_int, c_int, _P], c_int)
+
+
+def _dp(t):
+    """Address of a tensor for a ctypes pointer argument (None: null)."""
+    return None if t is None else t.data_ptr()
+
+
+def _launch(device, fn, *args):
+    """``fn(*args, stream)`` on the current stream of ``device`` — which need not be the current device."""
+    if device.index == torch.cuda.current_device():
+        return fn(*args, torch.cuda.current_stream().cuda_stream)
+    with torch.cuda.device(device):
+        return fn(*args, torch.cuda.current_stream().cuda_stream)
+
+
+def is_channels_last(t: torch.Tensor) -> bool:
+    """Does ``t [N, C, *]`` lie in memory as ``[N, *, C]``, dense?"""
+    d = t.dim()
+    if d == 4:
+        return t.is_contiguous(memory_format=torch.channels_last)
+    return t.is_contiguous() if d == 2 else t.movedim(1, -1).is_contiguous()
+
+
+def to_channels_last(t: torch.Tensor) -> torch.Tensor:
+    return t if is_channels_last(t) else t.movedim(1, -1).contiguous().movedim(-1, 1)
+
+
+def _vec_of(C: int, esize: int, *tensors) -> int:
+    """Elements per access: 16 bytes where the channel count and every address allow it, else 1."""
+    w = 16 // esize
+    if C % w:
+        return 1
+    for t in tensors:
+        if t is not None and t.data_ptr() % 16:
+            return 1
+    return w
+
+
+def _gn_plan(N, P, C, G, dt, vec, direction, what):
+    """(elements per access, workspace bytes)."""
+    ws = _gn_ws(N, P, C, G, dt, vec, direction)
+    if ws < 0 and vec > 1:  # wide groups of an odd number of channels
+        vec = 1
+        ws = _gn_ws(N, P, C, G, dt, vec, direction)
+    if ws < 0:
+        raise ValueError(f"{what}: {C} channels in {G} groups over {P} pixels are not supported (a group has at most 2048 "
+                         f"channels; 1024 where its channels or an address rule out 16-byte accesses)")
+    return vec, ws
+
+
+def group_norm_supported(x: torch.Tensor, groups: int) -> bool:
+    if _gn_ws is None or not (x.is_cuda and x.dtype in _DT_CODE and x.dim() >= 2 and x.numel() > 0):
+        return False
+    N, C = x.shape[0], x.shape[1]
+    return C % groups == 0 and _gn_ws(N, x.numel() // (N * C), C, groups, _DT_CODE[x.dtype], 1, 1) >= 0
+
+
+def _gn_check(name, x, C, K, device, **named):
+    for n, t in named.items():
+        if t is None:
+            continue
+        if t.device != device:
+            raise ValueError(f"{name}: {n} lives on {t.device}, x on {device}")
+        if n in ("weight", "bias"):
+            if not (t.dtype == torch.float32 and (tuple(t.shape) == (C,) or tuple(t.shape) == (K, C)) and t.stride(-1) == 1):
+                raise ValueError(f"{name}: {n} must be fp32 [{C}] or [{K}, {C}] with contiguous channels, got {t.dtype} "
+                                 f"{tuple(t.shape)} strides {t.stride()}")
+        elif t.shape != x.shape or t.dtype != x.dtype:
+            raise ValueError(f"{name}: {n} must match x ({x.dtype} {tuple(x.shape)}), got {t.dtype} {tuple(t.shape)}")
+
+
+def _gn_stride(t) -> int:
+    return 0 if t is None or t.dim() == 1 else t.stride(0)
+
+
+def group_norm_forward(x, groups: int, weight, bias, eps: float, act: str = "none", residual=None, clients: int = 1,
+                       want_gate: bool = False):
+    """``act(group_norm(x) * weight + bias + residual)`` for channels-last ``x [N, C, *]`` (fp32, bf16 or fp16).
+    ``weight`` / ``bias``: fp32 ``[C]`` or ``[clients, C]`` (any client stride).  Returns (y, stats, gate): stats
+    ``[2, N, groups]`` (mean, 1 / std) and, for a ReLU behind a residual with ``want_gate``, its gate, one byte per
+    16-byte vector, which spares the backward pass the residual."""
+    if not (x.is_cuda and x.dtype in _DT_CODE and x.dim() >= 2 and x.numel() > 0):
+        raise ValueError(f"group_norm: expected a CUDA fp32 / bf16 / fp16 tensor [N, C, *], got {x.device} {x.dtype} "
+                         f"{tuple(x.shape)}")
+    dev = x.device
+    x = to_channels_last(x)
+    N, C = x.shape[0], x.shape[1]
+    if groups < 1 or C % groups or N % clients:
+        raise ValueError(f"group_norm: {C} channels / {groups} groups, {N} samples / {clients} clients do not divide")
+    _gn_check("group_norm", x, C, clients, dev, weight=weight, bias=bias, residual=residual)
+    residual = None if residual is None else to_channels_last(residual)
+    P = x.numel() // (N * C)
+    y = _empty_like(x)
+    if not is_channels_last(y):  # a shape whose strides empty_like does not keep
+        y = _empty([N] + list(x.shape[2:]) + [C], dtype=x.dtype, device=dev).movedim(-1, 1)
+    vec = _vec_of(C, x.element_size(), x, residual)
+    dt = _DT_CODE[x.dtype]
+    vec, ws_bytes = _gn_plan(N, P, C, groups, dt, vec, 0, "group_norm")
+    stats = _empty(2, N, groups, dtype=torch.float32, device=dev)
+    gate = None
+    if want_gate and act == "relu" and residual is not None:
+        gate = _empty(x.numel() // vec, dtype=torch.uint8, device=dev)
+    ws = _empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    rc = _launch(dev, _gn_fwd, _dp(x), _dp(residual), _dp(weight), _dp(bias), N, P, C, groups, eps, ACT_CODE[act],
+                 N // clients, _gn_stride(weight), _gn_stride(bias), _dp(y), _dp(gate), _dp(stats),
+                 stats.data_ptr() + 4 * N * groups, _dp(ws), dt, vec)
+    if rc != 0:
+        raise ValueError(f"group_norm: rejected (rc={rc})")
+    return y, stats, (gate, vec) if gate is not None else None
+
+
+def group_norm_backward(x, gy, groups: int, weight, bias, stats, act: str = "none", residual=None, gate=None, clients: int = 1,
+                        want_dx: bool = True, want_dres: bool = False, dweight=None, dbias=None, ld: int = 0, coef=None,
+                        accumulate: bool = False):
+    """Gradients of ``group_norm_forward``: returns (dx, dres).  ``dweight`` / ``dbias``: fp32 tensors whose first
+    elements start client 0's row of C sums, ``ld`` floats from row to row (a ``[clients, C]`` tensor, or columns of the
+    update matrix); they receive — ``accumulate``: are incremented by — ``coef[client]`` (None: 1) times the sums."""
+    dev = x.device
+    x = to_channels_last(x)
+    N, C = x.shape[0], x.shape[1]
+    if gy.shape != x.shape or gy.dtype != x.dtype or gy.device != dev:
+        raise ValueError("group_norm_backward: gy must match x")
+    gy = to_channels_last(gy)
+    P = x.numel() // (N * C)
+    _gn_check("group_norm_backward", x, C, clients, dev, weight=weight, bias=bias, residual=residual)
+    residual = None if residual is None else to_channels_last(residual)
+    if stats.device != dev or stats.dtype != torch.float32 or not stats.is_contiguous() or stats.numel() != 2 * N * groups \
+            or C % groups or N % clients:
+        raise ValueError("group_norm_backward: stats do not match")
+    for n, t in (("dweight", dweight), ("dbias", dbias)):
+        if t is not None and not (t.device == dev and t.dtype == torch.float32 and tuple(t.shape) == (clients, C)
+                                  and t.stride(1) == 1 and (clients == 1 or t.stride(0) == ld) and ld >= C):
+            raise ValueError(f"group_norm_backward: {n} must be fp32 [{clients}, {C}] with row stride ld")
+    if coef is not None:
+        coef = _vec(coef, clients, dev, name="coef")
+    dx = _empty_like(x) if want_dx else None
+    if dx is not None and not is_channels_last(dx):
+        dx = _empty([N] + list(x.shape[2:]) + [C], dtype=x.dtype, device=dev).movedim(-1, 1)
+    dres = torch.empty_like(dx if dx is not None else x) if want_dres else None
+    vec = _vec_of(C, x.element_size(), x, gy, residual)
+    if gate is not None:
+        gate, gvec = gate
+        if gate.numel() * gvec != x.numel() or gate.device != dev:
+            raise ValueError("group_norm_backward: the gate does not match x")
+        if gvec != vec:  # the forward pass had 16-byte addresses and this gradient has not (or the other way round)
+            if gvec > vec:
+                gy = gy.clone(memory_format=torch.preserve_format)
+                x = x if x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.preserve_format)
+                residual, vec = None, gvec
+            else:
+                vec = gvec
+        residual = None
+    dt = _DT_CODE[x.dtype]
+    vec, ws_bytes = _gn_plan(N, P, C, groups, dt, vec, 1, "group_norm_backward")
+    ws = _empty(ws_bytes, dtype=torch.uint8, device=dev)
+    rc = _launch(dev, _gn_bwd, _dp(x), _dp(residual), _dp(gy), _dp(gate), _dp(weight), _dp(bias), _dp(stats),
+                 stats.data_ptr() + 4 * N * groups, N, P, C, groups, ACT_CODE[act], N // clients, _gn_stride(weight),
+                 _gn_stride(bias), _dp(dx), _dp(dres), _dp(coef), _dp(dweight), _dp(dbias), ld, int(accumulate), _dp(ws), dt,
+                 vec)
+    if rc != 0:
+        raise ValueError(f"group_norm_backward: rejected (rc={rc})")
+    return dx, dres
+
+
+def dropout_scale(p: float) -> float:
+    """1 / (1 - p) as the kernels compute it: in 32 bits."""
+    q = c_float(1.0 - c_float(p).value).value
+    return c_float(1.0 / q).value
+
+
+def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "elem", layout: str = "major", scale=None):
+    """``x`` times its client-keyed dropout multipliers (see reference.client_dropout), nothing stored.  ``tag``: an int,
+    or a 1-element int64 tensor read when the kernel runs (captured graphs)."""
+    if not (x.is_cuda and x.dtype in _DT_CODE and x.dim() >= 1):
+        raise ValueError(f"client_dropout: expected a CUDA fp32 / bf16 / fp16 tensor, got {x.device} {x.dtype}")
+    dev = x.device
+    if not (uids.device == dev and uids.dtype == torch.int64 and uids.dim() == 1 and uids.is_contiguous()):
+        raise ValueError("client_dropout: uids must be a contiguous int64 vector on x's device")
+    tag_value = 0
+    if torch.is_tensor(tag):
+        if not (tag.device == dev and tag.dtype == torch.int64 and tag.numel() == 1):
+            raise ValueError("client_dropout: tag must be an int or a 1-element int64 tensor on x's device")
+    else:
+        tag, tag_value = None, int(tag)
+    if x.numel() == 0:
+        return x.clone()
+    Kc = uids.numel()
+    shape = x.shape
+    if layout == "major":
+        B, C = shape[0] // Kc, (shape[1] if x.dim() > 1 else 1)
+    else:
+        B, C = shape[0], shape[1] // Kc
+    HW = x.numel() // (Kc * B * C)
+    last = x.dim() == 4 and not x.is_contiguous() and x.is_contiguous(memory_format=torch.channels_last)
+    if not last:
+        x = x.contiguous()
+    y = _empty_like(x)
+    vec = int(x.data_ptr() % 16 == 0 and y.data_ptr() % 16 == 0)
+    p32 = c_float(p).value
+    kinds = {"elem": 0, "channel": 1 if x.dim() > 2 else 0, "sample": 2}
+    rc = _launch(dev, _client_drop, _dp(x), _dp(y), _dp(uids), _dp(tag), tag_value, Kc, B, C, HW, kinds[kind],
+                 int(layout == "inner"), int(last), (2 + 256 * layer) & 0xFFFFFFFF, seed & (2 ** 64 - 1),
+                 _ceil(p32 * 16777216.0), dropout_scale(p) if scale is None else scale, _DT_CODE[x.dtype], vec)
+    if rc != 0:
+        raise ValueError(f"client_dropout: rejected (rc={rc}): a client's share of a layer has at most 1.7e10 elements")
+    return y
+
+
+def rope_axes(x, pos, axes, base: float = 10000.0, slots=None, inverse: bool = False, out=None):
+    """Rotary positions with several axes (see reference.rope_axes).  ``x`` may have any strides (last dimension
+    contiguous).  ``out``: None for a new contiguous tensor, or ``x`` itself: turned in place, other slots untouched."""
+    if not (x.is_cuda and x.dtype in _DT_CODE and x.dim() in (4, 5)):
+        raise ValueError(f"rope_axes: expected a CUDA fp32 / bf16 / fp16 tensor [R, N, H, D] or [R, N, S, H, D], got "
+                         f"{x.device} {x.dtype} {tuple(x.shape)}")
+    dev = x.device
+    R, N, H, D = x.shape[0], x.shape[1], x.shape[-2], x.shape[-1]
+    S = x.shape[2] if x.dim() == 5 else 1
+    rot = S if slots is None else int(slots)
+    axes = [int(a) for a in axes]
+    if not axes or len(axes) > 8 or any(a < 2 or a % 2 for a in axes) or sum(axes) > D or D % 2 or D > 256:
+        raise ValueError(f"rope_axes: sections {axes} must be even and fit the head dimension {D} (even, at most 256)")
+    if not 0 <= rot <= S or not base > 0.0:
+        raise ValueError(f"rope_axes: {rot} of {S} slots, base {base}")
+    if pos.device != dev or pos.dtype not in (torch.int64, torch.float32) or tuple(pos.shape) not in (
+            (N, len(axes)), (R, N, len(axes))):
+        raise ValueError(f"rope_axes: pos must be int64 or fp32 [{N}, {len(axes)}] or [{R}, {N}, {len(axes)}] on x's device, "
+                         f"got {pos.dtype} {tuple(pos.shape)} on {pos.device}")
+    if out is not None and out is not x:
+        raise ValueError("rope_axes: out must be x itself")
+    pos = pos.contiguous()
+    if x.stride(-1) != 1 and x.numel():
+        if out is not None:
+            raise ValueError("rope_axes: in place needs a contiguous last dimension")
+        x = x.contiguous()
+    if out is not None and not _no_overlap(x):
+        raise ValueError("rope_axes: in place needs a tensor without overlapping elements")
+    y = x if out is not None else _empty(x.shape, dtype=x.dtype, device=dev)
+    if x.numel() == 0:
+        return y
+    st = x.stride()
+    sr, sn, ss, sh = st[0], st[1], (st[2] if x.dim() == 5 else 0), st[-2]
+    w = 16 // x.element_size()
+    wide = D % w == 0 and x.data_ptr() % 16 == 0 and y.data_ptr() % 16 == 0 and not any(s % w for s in (sr, sn, ss, sh))
+    if not wide and (any(s % 2 for s in (sr, sn, ss, sh)) or x.data_ptr() % (2 * x.element_size())):
+        if out is not None:
+            raise ValueError("rope_axes: in place needs pairs at even addresses")
+        return rope_axes(x.clone(memory_format=torch.contiguous_format), pos, axes, base, slots, inverse)
+    rc = _launch(dev, _rope, _dp(x), _dp(y), _dp(pos), int(pos.dtype == torch.float32),
+                 N * len(axes) if pos.dim() == 3 else 0, R, N, S, H, D, sr, sn, ss, sh, rot, (c_int * len(axes))(*axes),
+                 len(axes), float(base), int(inverse), _DT_CODE[x.dtype], w if wide else 2)
+    if rc != 0:
+        raise ValueError(f"rope_axes: rejected (rc={rc})")
+    return y
+
+
+def _no_overlap(t) -> bool:
+    """Distinct elements at distinct addresses (sorted strides, each at least the extent of the smaller ones)."""
+    need = 1
+    for s, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if s < need:
+            return False
+        need = s * n
+    return True

@@ -18,6 +18,9 @@ HOST_LIB = HERE / "libblades_host.so"
 HIP_LIB = HERE / "libblades_hip.so"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
+# scalar fp32 instructions only: some forms of the packed ones (v_pk_fma_f32 and its like), which -O3 makes of ordinary
+# float code by itself, have given wrong results now and then (the host pass warns that it does not know the feature)
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _stale(target: Path, sources) -> bool:
@@ -53,7 +56,7 @@ def build_hip(force: bool = False, verbose: bool = False, jobs: int = 4) -> Path
         objs.append(o)
         if force or _stale(o, [s] + hdrs):
             cmd = [HIPCC, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-c", str(s), "-o", str(o),
-                   "-I", str(CSRC), "-Wno-unused-result"]
+                   "-I", str(CSRC), "-Wno-unused-result"] + NO_PACKED_FP32
             if verbose:
                 print(" ".join(cmd), flush=True)
             procs.append((s, subprocess.Popen(cmd)))

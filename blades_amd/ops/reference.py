@@ -9,6 +9,7 @@ and on the GPU test tier they are what each kernel is compared against.
 parameter coordinate; ``Dl`` is the local column shard).  ``mask`` is an
 optional ``[K]`` tensor; rows with ``mask == 0`` do not take part.
 """
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -421,3 +422,77 @@ def shuffle_keys(uids, epochs, lens, nmax: int, seed: int):
     w = _philox4x32(pos, uid & _MASK, ep & _MASK, torch.full_like(pos, 7), seed & _MASK, (seed >> 32) & _MASK)
     keys = (w[0] * 4294967296 + w[1]).double() / float(2 ** 64)
     return keys.masked_fill(pos >= lens.reshape(-1, 1), 2.0)
+
+
+def group_norm(x, groups: int, weight=None, bias=None, eps: float = 1e-5, act: str = "none", residual=None):
+    """Oracle of ops/csrc/groupnorm.hip: ``act(group_norm(x) * weight + bias + residual)`` for ``x [N, C, *]``;
+    ``weight`` / ``bias`` ``[C]``, or ``[K, C]`` for K clients of N / K consecutive samples each.  32-bit arithmetic
+    (64 for 64-bit inputs), rounded once.  Differentiable (plain torch ops)."""
+    acc = torch.float64 if x.dtype == torch.float64 else torch.float32
+    N, C = x.shape[0], x.shape[1]
+    tail = [1] * (x.dim() - 2)
+    xf = x.to(acc).reshape(N, groups, (C // groups) * math.prod(x.shape[2:]))
+    d = xf - xf.mean(dim=2, keepdim=True)
+    z = (d * torch.rsqrt(d.square().mean(dim=2, keepdim=True) + eps)).reshape(x.shape)
+
+    def per_sample(t):
+        t = t.to(acc)
+        return t.reshape(1, C, *tail) if t.dim() == 1 else t.repeat_interleave(N // t.shape[0], dim=0).reshape(N, C, *tail)
+
+    if weight is not None:
+        z = z * per_sample(weight)
+    if bias is not None:
+        z = z + per_sample(bias)
+    if residual is not None:
+        z = z + residual.to(acc)
+    F = torch.nn.functional
+    y = {"none": lambda t: t, "relu": F.relu, "gelu": F.gelu, "silu": F.silu}[act](z)
+    return y.to(x.dtype)
+
+
+def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "elem", layout: str = "major", scale=None):
+    """Oracle of ops/csrc/dropout.hip: ``x`` times the multipliers of ``client_dropout_mult``, laid over the elements,
+    channels or samples of every client's share of the batch.  Differentiable."""
+    uids = uids.reshape(-1)
+    Kc = uids.numel()
+    keep = 1 if kind == "sample" else (2 if kind == "channel" and x.dim() > 2 else x.dim())
+    if layout == "major":
+        lead, B, C = [Kc, x.shape[0] // Kc], x.shape[0] // Kc, (x.shape[1] if x.dim() > 1 else 1)
+    else:
+        lead, B, C = [x.shape[0], Kc], x.shape[0], x.shape[1] // Kc
+    value = [1 if i >= keep else (C if i == 1 else int(d)) for i, d in enumerate(x.shape)][1:]  # draws of one sample
+    n = B
+    for d in value:
+        n *= d
+    m = client_dropout_mult(uids, n, seed, tag, layer, p)
+    if scale is not None:
+        m = (m != 0).to(m.dtype) * scale
+    m = m.reshape([Kc, B] + value)
+    m = (m if layout == "major" else m.transpose(0, 1))
+    acc = torch.float64 if x.dtype == torch.float64 else torch.float32
+    xs = x.to(acc).reshape(lead + [C] * (x.dim() > 1) + list(x.shape[2:]))
+    return (xs * m.to(acc)).reshape(x.shape).to(x.dtype)
+
+
+def rope_axes(x, pos, axes, base: float = 10000.0, slots=None, inverse: bool = False):
+    """Oracle of ops/csrc/rope.hip: rotary positions with one section of the head dimension per axis.
+    ``x [R, N, H, D]``, or ``[R, N, S, H, D]`` whose first ``slots`` slots are turned; ``pos [N, A]`` or ``[R, N, A]``.
+    Angles in 64 bits, products in 32.  Differentiable."""
+    acc = torch.float64 if x.dtype == torch.float64 else torch.float32
+    dev = x.device
+    freq = torch.cat([float(base) ** (torch.arange(a // 2, dtype=torch.float64, device=dev) * (-2.0 / a)) for a in axes])
+    axis = torch.cat([torch.full((a // 2,), i, dtype=torch.int64, device=dev) for i, a in enumerate(axes)])
+    angle = pos.to(dev).double()[..., axis] * freq
+    cos, sin = angle.cos().to(acc).unsqueeze(-2), angle.sin().to(acc).unsqueeze(-2)
+    sin = -sin if inverse else sin
+    part, rest = x, None
+    if x.dim() == 5:
+        cos, sin = cos.unsqueeze(-3), sin.unsqueeze(-3)
+        if slots is not None and slots < x.shape[2]:
+            part, rest = x[:, :, :slots], x[:, :, slots:]
+    rot = 2 * freq.numel()
+    pf = part.to(acc)
+    a, b = pf[..., 0:rot:2], pf[..., 1:rot:2]
+    y = torch.stack((a * cos - b * sin, a * sin + b * cos), dim=-1).flatten(-2)
+    y = torch.cat((y, pf[..., rot:]), dim=-1).to(x.dtype)
+    return y if rest is None else torch.cat((y, rest), dim=2)
