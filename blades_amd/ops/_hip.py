@@ -10,6 +10,7 @@ Importing this module without the built library raises — GPU tensors never
 fall back to a PyTorch implementation.
 """
 import ctypes
+import functools
 from ctypes import c_double, c_float, c_int, c_long, c_uint, c_ulonglong, c_void_p
 from math import ceil as _ceil
 from typing import Optional
@@ -1802,12 +1803,15 @@ def _dp(t):
     return None if t is None else t.data_ptr()
 
 
-def _launch(device, fn, *args):
-    """``fn(*args, stream)`` on the current stream of ``device`` — which need not be the current device."""
-    if device.index == torch.cuda.current_device():
-        return fn(*args, torch.cuda.current_stream().cuda_stream)
-    with torch.cuda.device(device):
-        return fn(*args, torch.cuda.current_stream().cuda_stream)
+_raw_stream, _device_now = torch._C._cuda_getCurrentRawStream, torch.cuda.current_device
+
+
+def _launch(index: int, fn, *args):
+    """``fn(*args, stream)`` on the current stream of device ``index`` — which need not be the current device."""
+    if index == _device_now():
+        return fn(*args, _raw_stream(index))
+    with torch.cuda.device(index):
+        return fn(*args, _raw_stream(index))
 
 
 def is_channels_last(t: torch.Tensor) -> bool:
@@ -1822,48 +1826,62 @@ def to_channels_last(t: torch.Tensor) -> torch.Tensor:
     return t if is_channels_last(t) else t.movedim(1, -1).contiguous().movedim(-1, 1)
 
 
-def _vec_of(C: int, esize: int, *tensors) -> int:
-    """Elements per access: 16 bytes where the channel count and every address allow it, else 1."""
-    w = 16 // esize
-    if C % w:
-        return 1
-    for t in tensors:
-        if t is not None and t.data_ptr() % 16:
-            return 1
-    return w
+def _like_channels_last(x):
+    """An uninitialised tensor that lies as the channels-last ``x`` does."""
+    y = _empty_like(x)
+    if is_channels_last(y):
+        return y
+    return _empty([x.shape[0]] + list(x.shape[2:]) + [x.shape[1]], dtype=x.dtype, device=x.device).movedim(-1, 1)
 
 
-def _gn_plan(N, P, C, G, dt, vec, direction, what):
-    """(elements per access, workspace bytes)."""
+@functools.lru_cache(maxsize=4096)
+def _gn_plan(N, P, C, G, dt, vec, direction):
+    """(channels per access, workspace bytes) of a shape; workspace -1: not supported."""
     ws = _gn_ws(N, P, C, G, dt, vec, direction)
     if ws < 0 and vec > 1:  # wide groups of an odd number of channels
         vec = 1
         ws = _gn_ws(N, P, C, G, dt, vec, direction)
-    if ws < 0:
-        raise ValueError(f"{what}: {C} channels in {G} groups over {P} pixels are not supported (a group has at most 2048 "
-                         f"channels; 1024 where its channels or an address rule out 16-byte accesses)")
     return vec, ws
+
+
+def _gn_layout(x, G, direction, other, residual):
+    """(N, P, C, dtype code, channels per access, workspace bytes): four channels where their count and every address
+    allow them."""
+    N, C = x.shape[0], x.shape[1]
+    P = x.numel() // (N * C)
+    dt = _DT_CODE[x.dtype]
+    a = x.data_ptr() | (0 if other is None else other.data_ptr()) | (0 if residual is None else residual.data_ptr())
+    w = 1 if C % 4 or a % (16 if dt == 0 else 8) else 4
+    vec, ws = _gn_plan(N, P, C, G, dt, w, direction)
+    if ws < 0:
+        raise ValueError(f"group_norm: {C} channels in {G} groups over {P} pixels are not supported (a group has at most 2048 "
+                         f"channels; 1024 where C or an address rules out accesses of four)")
+    return N, P, C, dt, vec, ws
 
 
 def group_norm_supported(x: torch.Tensor, groups: int) -> bool:
     if _gn_ws is None or not (x.is_cuda and x.dtype in _DT_CODE and x.dim() >= 2 and x.numel() > 0):
         return False
     N, C = x.shape[0], x.shape[1]
-    return C % groups == 0 and _gn_ws(N, x.numel() // (N * C), C, groups, _DT_CODE[x.dtype], 1, 1) >= 0
+    return C % groups == 0 and _gn_plan(N, x.numel() // (N * C), C, groups, _DT_CODE[x.dtype], 1, 1)[1] >= 0
 
 
-def _gn_check(name, x, C, K, device, **named):
-    for n, t in named.items():
-        if t is None:
-            continue
-        if t.device != device:
-            raise ValueError(f"{name}: {n} lives on {t.device}, x on {device}")
-        if n in ("weight", "bias"):
-            if not (t.dtype == torch.float32 and (tuple(t.shape) == (C,) or tuple(t.shape) == (K, C)) and t.stride(-1) == 1):
-                raise ValueError(f"{name}: {n} must be fp32 [{C}] or [{K}, {C}] with contiguous channels, got {t.dtype} "
-                                 f"{tuple(t.shape)} strides {t.stride()}")
-        elif t.shape != x.shape or t.dtype != x.dtype:
-            raise ValueError(f"{name}: {n} must match x ({x.dtype} {tuple(x.shape)}), got {t.dtype} {tuple(t.shape)}")
+def _gn_check(name, x, groups, clients, weight, bias, *others):
+    if not (x.is_cuda and x.dtype in _DT_CODE and x.dim() >= 2 and x.numel() > 0):
+        raise ValueError(f"{name}: expected a CUDA fp32 / bf16 / fp16 tensor [N, C, *], got {x.device} {x.dtype} "
+                         f"{tuple(x.shape)}")
+    N, C = x.shape[0], x.shape[1]
+    if groups < 1 or C % groups or clients < 1 or N % clients:
+        raise ValueError(f"{name}: {C} channels / {groups} groups, {N} samples / {clients} clients do not divide")
+    for t in (weight, bias):
+        if t is not None and not (t.dtype == torch.float32 and t.device == x.device and t.stride(-1) == 1
+                                  and (t.shape == (C,) or t.shape == (clients, C))):
+            raise ValueError(f"{name}: weight and bias must be fp32 [{C}] or [{clients}, {C}] with contiguous channels on "
+                             f"{x.device}, got {t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}")
+    for t in others:
+        if t is not None and (t.shape != x.shape or t.dtype != x.dtype or t.device != x.device):
+            raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device} does not match x, {x.dtype} {tuple(x.shape)} "
+                             f"on {x.device}")
 
 
 def _gn_stride(t) -> int:
@@ -1871,89 +1889,73 @@ def _gn_stride(t) -> int:
 
 
 def group_norm_forward(x, groups: int, weight, bias, eps: float, act: str = "none", residual=None, clients: int = 1,
-                       want_gate: bool = False):
+                       for_backward: bool = True, checked: bool = False):
     """``act(group_norm(x) * weight + bias + residual)`` for channels-last ``x [N, C, *]`` (fp32, bf16 or fp16).
-    ``weight`` / ``bias``: fp32 ``[C]`` or ``[clients, C]`` (any client stride).  Returns (y, stats, gate): stats
-    ``[2, N, groups]`` (mean, 1 / std) and, for a ReLU behind a residual with ``want_gate``, its gate, one byte per
-    16-byte vector, which spares the backward pass the residual."""
-    if not (x.is_cuda and x.dtype in _DT_CODE and x.dim() >= 2 and x.numel() > 0):
-        raise ValueError(f"group_norm: expected a CUDA fp32 / bf16 / fp16 tensor [N, C, *], got {x.device} {x.dtype} "
-                         f"{tuple(x.shape)}")
-    dev = x.device
+    ``weight`` / ``bias``: fp32 ``[C]`` or ``[clients, C]`` (any client stride).  Returns (y, stats, gate).  For a backward
+    pass: stats ``[2, N, groups]`` (mean, 1 / std) and, for a ReLU behind a residual, its gate, one byte per vector, which
+    spares that pass the residual: (bytes, elements per vector); else None.  ``checked``: the caller did."""
+    if not checked:
+        _gn_check("group_norm", x, groups, clients, weight, bias, residual)
     x = to_channels_last(x)
-    N, C = x.shape[0], x.shape[1]
-    if groups < 1 or C % groups or N % clients:
-        raise ValueError(f"group_norm: {C} channels / {groups} groups, {N} samples / {clients} clients do not divide")
-    _gn_check("group_norm", x, C, clients, dev, weight=weight, bias=bias, residual=residual)
     residual = None if residual is None else to_channels_last(residual)
-    P = x.numel() // (N * C)
-    y = _empty_like(x)
-    if not is_channels_last(y):  # a shape whose strides empty_like does not keep
-        y = _empty([N] + list(x.shape[2:]) + [C], dtype=x.dtype, device=dev).movedim(-1, 1)
-    vec = _vec_of(C, x.element_size(), x, residual)
-    dt = _DT_CODE[x.dtype]
-    vec, ws_bytes = _gn_plan(N, P, C, groups, dt, vec, 0, "group_norm")
-    stats = _empty(2, N, groups, dtype=torch.float32, device=dev)
-    gate = None
-    if want_gate and act == "relu" and residual is not None:
+    N, P, C, dt, vec, ws_bytes = _gn_layout(x, groups, 0, None, residual)
+    dev = x.device
+    y = _like_channels_last(x)
+    stats = gate = ws = None
+    mean = rstd = None
+    if for_backward or ws_bytes:
+        stats = _empty(2, N, groups, dtype=torch.float32, device=dev)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * N * groups
+    if for_backward and residual is not None and act == "relu":
         gate = _empty(x.numel() // vec, dtype=torch.uint8, device=dev)
-    ws = _empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-    rc = _launch(dev, _gn_fwd, _dp(x), _dp(residual), _dp(weight), _dp(bias), N, P, C, groups, eps, ACT_CODE[act],
-                 N // clients, _gn_stride(weight), _gn_stride(bias), _dp(y), _dp(gate), _dp(stats),
-                 stats.data_ptr() + 4 * N * groups, _dp(ws), dt, vec)
+    if ws_bytes:
+        ws = _empty(ws_bytes, dtype=torch.uint8, device=dev)
+    rc = _launch(dev.index, _gn_fwd, x.data_ptr(), _dp(residual), _dp(weight), _dp(bias), N, P, C, groups, eps, ACT_CODE[act],
+                 N // clients, _gn_stride(weight), _gn_stride(bias), y.data_ptr(), _dp(gate), mean, rstd, _dp(ws), dt, vec)
     if rc != 0:
         raise ValueError(f"group_norm: rejected (rc={rc})")
-    return y, stats, (gate, vec) if gate is not None else None
+    return y, stats, None if gate is None else (gate, vec)
 
 
 def group_norm_backward(x, gy, groups: int, weight, bias, stats, act: str = "none", residual=None, gate=None, clients: int = 1,
                         want_dx: bool = True, want_dres: bool = False, dweight=None, dbias=None, ld: int = 0, coef=None,
-                        accumulate: bool = False):
-    """Gradients of ``group_norm_forward``: returns (dx, dres).  ``dweight`` / ``dbias``: fp32 tensors whose first
-    elements start client 0's row of C sums, ``ld`` floats from row to row (a ``[clients, C]`` tensor, or columns of the
-    update matrix); they receive — ``accumulate``: are incremented by — ``coef[client]`` (None: 1) times the sums."""
-    dev = x.device
-    x = to_channels_last(x)
-    N, C = x.shape[0], x.shape[1]
-    if gy.shape != x.shape or gy.dtype != x.dtype or gy.device != dev:
-        raise ValueError("group_norm_backward: gy must match x")
-    gy = to_channels_last(gy)
-    P = x.numel() // (N * C)
-    _gn_check("group_norm_backward", x, C, clients, dev, weight=weight, bias=bias, residual=residual)
-    residual = None if residual is None else to_channels_last(residual)
-    if stats.device != dev or stats.dtype != torch.float32 or not stats.is_contiguous() or stats.numel() != 2 * N * groups \
-            or C % groups or N % clients:
-        raise ValueError("group_norm_backward: stats do not match")
-    for n, t in (("dweight", dweight), ("dbias", dbias)):
-        if t is not None and not (t.device == dev and t.dtype == torch.float32 and tuple(t.shape) == (clients, C)
-                                  and t.stride(1) == 1 and (clients == 1 or t.stride(0) == ld) and ld >= C):
-            raise ValueError(f"group_norm_backward: {n} must be fp32 [{clients}, {C}] with row stride ld")
-    if coef is not None:
-        coef = _vec(coef, clients, dev, name="coef")
-    dx = _empty_like(x) if want_dx else None
-    if dx is not None and not is_channels_last(dx):
-        dx = _empty([N] + list(x.shape[2:]) + [C], dtype=x.dtype, device=dev).movedim(-1, 1)
-    dres = torch.empty_like(dx if dx is not None else x) if want_dres else None
-    vec = _vec_of(C, x.element_size(), x, gy, residual)
-    if gate is not None:
-        gate, gvec = gate
-        if gate.numel() * gvec != x.numel() or gate.device != dev:
+                        accumulate: bool = False, checked: bool = False):
+    """Gradients of ``group_norm_forward``: returns (dx, dres).  ``dweight`` / ``dbias``: fp32 ``[clients, C]`` tensors, rows
+    ``ld`` floats apart (columns of the update matrix, for one); they receive — ``accumulate``: are incremented by —
+    ``coef[client]`` (None: 1) times the sums.  ``gate``: as the forward pass returned it, in place of the residual."""
+    if not checked:
+        _gn_check("group_norm_backward", x, groups, clients, weight, bias, gy, residual)
+        N, C = x.shape[0], x.shape[1]
+        if stats.device != x.device or stats.dtype != torch.float32 or not stats.is_contiguous() \
+                or stats.numel() != 2 * N * groups:
+            raise ValueError("group_norm_backward: stats do not match")
+        for n, t in (("dweight", dweight), ("dbias", dbias)):
+            if t is not None and not (t.device == x.device and t.dtype == torch.float32 and tuple(t.shape) == (clients, C)
+                                      and t.stride(1) == 1 and (clients == 1 or t.stride(0) == ld) and ld >= C):
+                raise ValueError(f"group_norm_backward: {n} must be fp32 [{clients}, {C}] with row stride ld")
+        if coef is not None:
+            coef = _vec(coef, clients, x.device, name="coef")
+        if gate is not None and (gate[0].numel() * gate[1] != x.numel() or gate[0].device != x.device):
             raise ValueError("group_norm_backward: the gate does not match x")
-        if gvec != vec:  # the forward pass had 16-byte addresses and this gradient has not (or the other way round)
-            if gvec > vec:
-                gy = gy.clone(memory_format=torch.preserve_format)
-                x = x if x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.preserve_format)
-                residual, vec = None, gvec
-            else:
-                vec = gvec
-        residual = None
-    dt = _DT_CODE[x.dtype]
-    vec, ws_bytes = _gn_plan(N, P, C, groups, dt, vec, 1, "group_norm_backward")
+    x, gy = to_channels_last(x), to_channels_last(gy)
+    residual = None if residual is None or gate is not None else to_channels_last(residual)
+    N, P, C, dt, vec, ws_bytes = _gn_layout(x, groups, 1, gy, residual)
+    bits = None
+    if gate is not None:
+        bits, gvec = gate
+        if gvec != vec:  # the gate's vectors decide: the two passes saw different alignments
+            if gvec > 1:
+                x, gy = (t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.preserve_format) for t in (x, gy))
+            vec, ws_bytes = _gn_plan(N, P, C, groups, dt, gvec, 1)
+    dev = x.device
+    dx = _like_channels_last(x) if want_dx else None
+    dres = _like_channels_last(x) if want_dres else None
     ws = _empty(ws_bytes, dtype=torch.uint8, device=dev)
-    rc = _launch(dev, _gn_bwd, _dp(x), _dp(residual), _dp(gy), _dp(gate), _dp(weight), _dp(bias), _dp(stats),
-                 stats.data_ptr() + 4 * N * groups, N, P, C, groups, ACT_CODE[act], N // clients, _gn_stride(weight),
-                 _gn_stride(bias), _dp(dx), _dp(dres), _dp(coef), _dp(dweight), _dp(dbias), ld, int(accumulate), _dp(ws), dt,
-                 vec)
+    mean = stats.data_ptr()
+    rc = _launch(dev.index, _gn_bwd, x.data_ptr(), _dp(residual), gy.data_ptr(), _dp(bits), _dp(weight), _dp(bias), mean,
+                 mean + 4 * N * groups, N, P, C, groups, ACT_CODE[act], N // clients, _gn_stride(weight), _gn_stride(bias),
+                 _dp(dx), _dp(dres), _dp(coef), _dp(dweight), _dp(dbias), ld, int(accumulate), ws.data_ptr(), dt, vec)
     if rc != 0:
         raise ValueError(f"group_norm_backward: rejected (rc={rc})")
     return dx, dres
@@ -1965,86 +1967,98 @@ def dropout_scale(p: float) -> float:
     return c_float(1.0 / q).value
 
 
-def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "elem", layout: str = "major", scale=None):
-    """``x`` times its client-keyed dropout multipliers (see reference.client_dropout), nothing stored.  ``tag``: an int,
-    or a 1-element int64 tensor read when the kernel runs (captured graphs)."""
-    if not (x.is_cuda and x.dtype in _DT_CODE and x.dim() >= 1):
-        raise ValueError(f"client_dropout: expected a CUDA fp32 / bf16 / fp16 tensor, got {x.device} {x.dtype}")
-    dev = x.device
-    if not (uids.device == dev and uids.dtype == torch.int64 and uids.dim() == 1 and uids.is_contiguous()):
-        raise ValueError("client_dropout: uids must be a contiguous int64 vector on x's device")
-    tag_value = 0
-    if torch.is_tensor(tag):
-        if not (tag.device == dev and tag.dtype == torch.int64 and tag.numel() == 1):
-            raise ValueError("client_dropout: tag must be an int or a 1-element int64 tensor on x's device")
-    else:
-        tag, tag_value = None, int(tag)
-    if x.numel() == 0:
-        return x.clone()
-    Kc = uids.numel()
-    shape = x.shape
+@functools.lru_cache(maxsize=4096)
+def _drop_plan(shape, Kc, kind, layout, last, layer, seed, p, scale, dt):
+    """The arguments of a client_dropout launch that its shape and key fix."""
     if layout == "major":
-        B, C = shape[0] // Kc, (shape[1] if x.dim() > 1 else 1)
+        B, C = shape[0] // Kc, (shape[1] if len(shape) > 1 else 1)
     else:
         B, C = shape[0], shape[1] // Kc
-    HW = x.numel() // (Kc * B * C)
-    last = x.dim() == 4 and not x.is_contiguous() and x.is_contiguous(memory_format=torch.channels_last)
-    if not last:
-        x = x.contiguous()
+    numel = 1
+    for d in shape:
+        numel *= d
+    code = {"elem": 0, "channel": 1 if len(shape) > 2 else 0, "sample": 2}[kind]
+    return (Kc, B, C, numel // (Kc * B * C), code, int(layout == "inner"), int(last), (2 + 256 * layer) & 0xFFFFFFFF,
+            seed & (2 ** 64 - 1), _ceil(c_float(p).value * 16777216.0), dropout_scale(p) if scale is None else scale, dt)
+
+
+def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "elem", layout: str = "major", scale=None,
+                   checked: bool = False):
+    """``x`` times its client-keyed dropout multipliers (see reference.client_dropout), nothing stored.  ``tag``: an int,
+    or a 1-element int64 tensor read when the kernel runs (captured graphs).  ``checked``: the caller did."""
+    if not checked:
+        if not (x.is_cuda and x.dtype in _DT_CODE and x.dim() >= 1):
+            raise ValueError(f"client_dropout: expected a CUDA fp32 / bf16 / fp16 tensor, got {x.device} {x.dtype}")
+        if not (uids.device == x.device and uids.dtype == torch.int64 and uids.dim() == 1 and uids.is_contiguous()
+                and uids.numel() > 0 and x.shape[1 if layout == "inner" else 0] % uids.numel() == 0):
+            raise ValueError("client_dropout: uids must be a contiguous int64 vector on x's device that divides the batch")
+        if torch.is_tensor(tag) and not (tag.device == x.device and tag.dtype == torch.int64 and tag.numel() == 1):
+            raise ValueError("client_dropout: tag must be an int or a 1-element int64 tensor on x's device")
+        if not 0.0 <= p < 1.0:
+            raise ValueError("client_dropout: need 0 <= p < 1")
+    if x.numel() == 0:
+        return x.clone()
+    last = False
+    if not x.is_contiguous():
+        last = x.dim() == 4 and x.is_contiguous(memory_format=torch.channels_last)
+        x = x if last else x.contiguous()
     y = _empty_like(x)
-    vec = int(x.data_ptr() % 16 == 0 and y.data_ptr() % 16 == 0)
-    p32 = c_float(p).value
-    kinds = {"elem": 0, "channel": 1 if x.dim() > 2 else 0, "sample": 2}
-    rc = _launch(dev, _client_drop, _dp(x), _dp(y), _dp(uids), _dp(tag), tag_value, Kc, B, C, HW, kinds[kind],
-                 int(layout == "inner"), int(last), (2 + 256 * layer) & 0xFFFFFFFF, seed & (2 ** 64 - 1),
-                 _ceil(p32 * 16777216.0), dropout_scale(p) if scale is None else scale, _DT_CODE[x.dtype], vec)
+    at, to = x.data_ptr(), y.data_ptr()
+    plan = _drop_plan(tuple(x.shape), uids.numel(), kind, layout, last, layer, seed, p, scale, _DT_CODE[x.dtype])
+    by_value = not torch.is_tensor(tag)
+    rc = _launch(x.device.index, _client_drop, at, to, uids.data_ptr(), None if by_value else tag.data_ptr(),
+                 tag if by_value else 0, *plan, int(at % 16 == 0 and to % 16 == 0))
     if rc != 0:
         raise ValueError(f"client_dropout: rejected (rc={rc}): a client's share of a layer has at most 1.7e10 elements")
     return y
 
 
-def rope_axes(x, pos, axes, base: float = 10000.0, slots=None, inverse: bool = False, out=None):
+@functools.lru_cache(maxsize=1024)
+def _c_ints(values):
+    return (c_int * len(values))(*values)
+
+
+def rope_axes(x, pos, axes, base: float = 10000.0, slots=None, inverse: bool = False, out=None, checked: bool = False):
     """Rotary positions with several axes (see reference.rope_axes).  ``x`` may have any strides (last dimension
-    contiguous).  ``out``: None for a new contiguous tensor, or ``x`` itself: turned in place, other slots untouched."""
-    if not (x.is_cuda and x.dtype in _DT_CODE and x.dim() in (4, 5)):
-        raise ValueError(f"rope_axes: expected a CUDA fp32 / bf16 / fp16 tensor [R, N, H, D] or [R, N, S, H, D], got "
-                         f"{x.device} {x.dtype} {tuple(x.shape)}")
-    dev = x.device
-    R, N, H, D = x.shape[0], x.shape[1], x.shape[-2], x.shape[-1]
-    S = x.shape[2] if x.dim() == 5 else 1
-    rot = S if slots is None else int(slots)
-    axes = [int(a) for a in axes]
-    if not axes or len(axes) > 8 or any(a < 2 or a % 2 for a in axes) or sum(axes) > D or D % 2 or D > 256:
-        raise ValueError(f"rope_axes: sections {axes} must be even and fit the head dimension {D} (even, at most 256)")
-    if not 0 <= rot <= S or not base > 0.0:
-        raise ValueError(f"rope_axes: {rot} of {S} slots, base {base}")
-    if pos.device != dev or pos.dtype not in (torch.int64, torch.float32) or tuple(pos.shape) not in (
-            (N, len(axes)), (R, N, len(axes))):
-        raise ValueError(f"rope_axes: pos must be int64 or fp32 [{N}, {len(axes)}] or [{R}, {N}, {len(axes)}] on x's device, "
-                         f"got {pos.dtype} {tuple(pos.shape)} on {pos.device}")
-    if out is not None and out is not x:
-        raise ValueError("rope_axes: out must be x itself")
+    contiguous).  ``out``: None for a new contiguous tensor, or ``x`` itself: turned in place, other slots untouched.
+    ``checked``: the caller did, and ``axes`` is a tuple of ints, ``slots`` an int."""
+    five = x.dim() == 5
+    R, N, D = x.shape[0], x.shape[1], x.shape[-1]
+    S, H = (x.shape[2], x.shape[3]) if five else (1, x.shape[2])
+    if not checked:
+        axes, slots = tuple(int(a) for a in axes), S if slots is None else int(slots)
+        if not (x.is_cuda and x.dtype in _DT_CODE and x.dim() in (4, 5)):
+            raise ValueError(f"rope_axes: expected a CUDA fp32 / bf16 / fp16 tensor [R, N, H, D] or [R, N, S, H, D], got "
+                             f"{x.device} {x.dtype} {tuple(x.shape)}")
+        if not axes or len(axes) > 8 or any(a < 2 or a % 2 for a in axes) or sum(axes) > D or D % 2 or D > 256:
+            raise ValueError(f"rope_axes: sections {axes} must be even and fit the head dimension {D} (even, at most 256)")
+        if not 0 <= slots <= S or not base > 0.0:
+            raise ValueError(f"rope_axes: {slots} of {S} slots, base {base}")
+        if pos.device != x.device or pos.dtype not in (torch.int64, torch.float32) or tuple(pos.shape) not in (
+                (N, len(axes)), (R, N, len(axes))):
+            raise ValueError(f"rope_axes: pos must be int64 or fp32 [{N}, {len(axes)}] or [{R}, {N}, {len(axes)}] on x's "
+                             f"device, got {pos.dtype} {tuple(pos.shape)} on {pos.device}")
+        if out is not None and (out is not x or x.stride(-1) != 1 or not _no_overlap(x)):
+            raise ValueError("rope_axes: out must be x itself, without overlapping elements, its last dimension contiguous")
     pos = pos.contiguous()
-    if x.stride(-1) != 1 and x.numel():
-        if out is not None:
-            raise ValueError("rope_axes: in place needs a contiguous last dimension")
-        x = x.contiguous()
-    if out is not None and not _no_overlap(x):
-        raise ValueError("rope_axes: in place needs a tensor without overlapping elements")
-    y = x if out is not None else _empty(x.shape, dtype=x.dtype, device=dev)
     if x.numel() == 0:
-        return y
+        return x if out is not None else _empty(x.shape, dtype=x.dtype, device=x.device)
+    if x.stride(-1) != 1:
+        x = x.contiguous()
+    dt = _DT_CODE[x.dtype]
+    w = 4 if dt == 0 else 8
     st = x.stride()
-    sr, sn, ss, sh = st[0], st[1], (st[2] if x.dim() == 5 else 0), st[-2]
-    w = 16 // x.element_size()
-    wide = D % w == 0 and x.data_ptr() % 16 == 0 and y.data_ptr() % 16 == 0 and not any(s % w for s in (sr, sn, ss, sh))
-    if not wide and (any(s % 2 for s in (sr, sn, ss, sh)) or x.data_ptr() % (2 * x.element_size())):
-        if out is not None:
-            raise ValueError("rope_axes: in place needs pairs at even addresses")
-        return rope_axes(x.clone(memory_format=torch.contiguous_format), pos, axes, base, slots, inverse)
-    rc = _launch(dev, _rope, _dp(x), _dp(y), _dp(pos), int(pos.dtype == torch.float32),
-                 N * len(axes) if pos.dim() == 3 else 0, R, N, S, H, D, sr, sn, ss, sh, rot, (c_int * len(axes))(*axes),
-                 len(axes), float(base), int(inverse), _DT_CODE[x.dtype], w if wide else 2)
+    sr, sn, ss, sh = st[0], st[1], st[2] if five else 0, st[-2]
+    if D % w or (sr | sn | ss | sh) % w or x.data_ptr() % 16:
+        w = 2
+        if (sr | sn | ss | sh) % 2 or x.data_ptr() % (2 * x.element_size()):
+            if out is not None:
+                raise ValueError("rope_axes: in place needs pairs at even addresses")
+            return rope_axes(x.clone(memory_format=torch.contiguous_format), pos, axes, base, slots, inverse, None, True)
+    y = x if out is not None else _empty(x.shape, dtype=x.dtype, device=x.device)
+    rc = _launch(x.device.index, _rope, x.data_ptr(), y.data_ptr(), pos.data_ptr(), int(pos.dtype == torch.float32),
+                 N * len(axes) if pos.dim() == 3 else 0, R, N, S, H, D, sr, sn, ss, sh, slots, _c_ints(axes), len(axes), base,
+                 int(inverse), dt, w)
     if rc != 0:
         raise ValueError(f"rope_axes: rejected (rc={rc})")
     return y

@@ -8,6 +8,7 @@ PyTorch headers: a full rebuild is seconds, and hipcc cross-compiles gfx950
 code objects on a machine without a GPU.
 """
 import os
+import re
 import subprocess
 import sys
 from pathlib import Path
@@ -40,13 +41,24 @@ def build_host(force: bool = False, verbose: bool = False) -> Path:
     return HOST_LIB
 
 
+def _headers(src: Path) -> list:
+    """The headers of ``csrc`` that a source includes, directly or through another."""
+    found, todo = [], [src]
+    while todo:
+        for name in re.findall(r'^#include "([^"]+)"', todo.pop().read_text(), re.M):
+            h = CSRC / name
+            if h.exists() and h not in found:
+                found.append(h)
+                todo.append(h)
+    return found
+
+
 def hip_sources():
     return sorted(CSRC.glob("*.hip"))
 
 
 def build_hip(force: bool = False, verbose: bool = False, jobs: int = 4) -> Path:
     srcs = hip_sources()
-    hdrs = list(CSRC.glob("*.h")) + list(CSRC.glob("*.hpp"))
     objdir = HERE / "_build"
     objdir.mkdir(exist_ok=True)
     procs = []
@@ -54,7 +66,7 @@ def build_hip(force: bool = False, verbose: bool = False, jobs: int = 4) -> Path
     for s in srcs:
         o = objdir / (s.stem + ".o")
         objs.append(o)
-        if force or _stale(o, [s] + hdrs):
+        if force or _stale(o, [s] + _headers(s)):
             cmd = [HIPCC, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-c", str(s), "-o", str(o),
                    "-I", str(CSRC), "-Wno-unused-result"] + NO_PACKED_FP32
             if verbose:

@@ -39,11 +39,13 @@ __device__ __forceinline__ unsigned keep4(const Key& key, uint32_t q, uint32_t u
 __device__ __forceinline__ uint32_t tag_of(const Key& key) { return (uint32_t)(key.tag ? key.tag[0] : key.tag_value); }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Contiguous blocks.  Block r holds `len` values of memory starting at r * len; they belong to client r % Kc (inner) or r
-// and are its elements e0 = (r / Kc) * len (inner) or 0 onwards.  A value is drawn for every `seg` elements (1: each).
-template <typename T, int VEC, bool SEG>
-__global__ __launch_bounds__(TPB) void drop_flat_kernel(Key key, const T* __restrict__ x, T* __restrict__ y, long nblk, int Kc,
-                                                        int inner, long len, long seg) {
+// A draw for every element of contiguous blocks.  Block r holds `len` values of memory starting at r * len; they belong to
+// client r % Kc (inner) or r and are its elements e0 = (r / Kc) * len (inner) or 0 onwards.  U vectors a thread are on their
+// way while the draws are made; VEC 1 (a share whose length is no multiple of a vector's): one draw of four a thread,
+// wherever the block starts inside it.
+template <typename T, int VEC, int U>
+__global__ __launch_bounds__(TPB) void drop_elem_kernel(Key key, const T* __restrict__ x, T* __restrict__ y, long nblk, int Kc,
+                                                        int inner, long len) {
   typedef Pack<T, VEC> V;
   const uint32_t tag = tag_of(key);
   for (long r = blockIdx.y; r < nblk; r += gridDim.y) {
@@ -51,54 +53,105 @@ __global__ __launch_bounds__(TPB) void drop_flat_kernel(Key key, const T* __rest
     const long e0 = inner ? r / Kc * len : 0;
     const T* xb = x + r * len;
     T* yb = y + r * len;
-    if (!SEG && VEC > 1) {
+    if (VEC > 1) {
       // e0 and len are multiples of VEC here: a vector is one or two whole draws of four
       const long nv = len / VEC;
-      for (long v = (long)blockIdx.x * TPB + threadIdx.x; v < nv; v += (long)gridDim.x * TPB) {
-        V w = reinterpret_cast<const V*>(xb)[v];
-        const uint32_t q = (uint32_t)((e0 + v * VEC) >> 2);
-        unsigned m = keep4(key, q, uid, tag);
-        if (VEC == 8) m |= keep4(key, q + 1, uid, tag) << 4;
+      for (long v0 = (long)blockIdx.x * TPB * U + threadIdx.x; v0 < nv; v0 += (long)gridDim.x * TPB * U) {
+        V w[U];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) from_f(to_f(w.e[j]) * ((m >> j) & 1u ? key.scale : 0.f), w.e[j]);
-        reinterpret_cast<V*>(yb)[v] = w;
-      }
-    } else if (!SEG) {
-      // one draw of four per thread, wherever the block starts inside it
-      const long q0 = e0 >> 2, nq = ((e0 + len - 1) >> 2) - q0 + 1;
-      for (long q = (long)blockIdx.x * TPB + threadIdx.x; q < nq; q += (long)gridDim.x * TPB) {
-        const unsigned m = keep4(key, (uint32_t)(q0 + q), uid, tag);
-        const long first = (q0 + q) * 4 - e0;
+        for (int u = 0; u < U; ++u)
+          if (v0 + u * TPB < nv) w[u] = reinterpret_cast<const V*>(xb)[v0 + u * TPB];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const long i = first + j;
-          if (i >= 0 && i < len) from_f(to_f(xb[i]) * ((m >> j) & 1u ? key.scale : 0.f), yb[i]);
-        }
+        for (int u = 0; u < U; ++u)
+          if (v0 + u * TPB < nv) {
+            const uint32_t q = (uint32_t)((e0 + (v0 + u * TPB) * VEC) >> 2);
+            unsigned m = keep4(key, q, uid, tag);
+            if (VEC == 8) m |= keep4(key, q + 1, uid, tag) << 4;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) from_f(to_f(w[u].e[j]) * ((m >> j) & 1u ? key.scale : 0.f), w[u].e[j]);
+            reinterpret_cast<V*>(yb)[v0 + u * TPB] = w[u];
+          }
       }
     } else {
-      // one draw per vector: seg is a multiple of VEC
-      const long nv = len / VEC;
-      for (long v = (long)blockIdx.x * TPB + threadIdx.x; v < nv; v += (long)gridDim.x * TPB) {
-        V w = reinterpret_cast<const V*>(xb)[v];
-        const long i = (e0 + v * VEC) / seg;
-        const float s = (keep4(key, (uint32_t)(i >> 2), uid, tag) >> (i & 3)) & 1u ? key.scale : 0.f;
+      const long q0 = e0 >> 2, nq = ((e0 + len - 1) >> 2) - q0 + 1;
+      for (long q = (long)blockIdx.x * TPB + threadIdx.x; q < nq; q += (long)gridDim.x * TPB) {
+        const long first = (q0 + q) * 4 - e0;
+        T w[4];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) from_f(to_f(w.e[j]) * s, w.e[j]);
-        reinterpret_cast<V*>(yb)[v] = w;
+        for (int j = 0; j < 4; ++j)
+          if (first + j >= 0 && first + j < len) w[j] = xb[first + j];
+        const unsigned m = keep4(key, (uint32_t)(q0 + q), uid, tag);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (first + j >= 0 && first + j < len) {
+            from_f(to_f(w[j]) * ((m >> j) & 1u ? key.scale : 0.f), w[j]);
+            yb[first + j] = w[j];
+          }
       }
     }
   }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Channels-last maps.  Sample b of client k: pixel p, channel c at base(b, k) + p * pitch + c.  The draws of CT channels x
-// PT pixels go to LDS first, one byte per draw of four — in the order they are counted in, pixels fastest — then the tile
-// is walked in memory order, VEC channels a thread.  kind 0: value (b * C + c) * HW + p; 1: b * C + c; 2: b.
+// A draw for every channel of a sample (kind 1) or every sample (2): every vector's thread makes its own, which costs less
+// than waiting for another's.  Memory is [..][dims], walked by vectors of VEC channels (LAST: [sample][pixel][client if
+// inner][C]) or of one channel's pixels (else: [sample][C][pixel]); index arithmetic in I bits.
+template <typename T, int VEC, bool LAST, typename I>
+__global__ __launch_bounds__(TPB) void drop_group_kernel(Key key, const T* __restrict__ x, T* __restrict__ y, int Kc, I B, I C,
+                                                         I HW, int inner, int kind, I total) {
+  typedef Pack<T, VEC> V;
+  constexpr int U = 2;
+  const uint32_t tag = tag_of(key);
+  for (I i0 = (I)blockIdx.x * (TPB * U) + threadIdx.x; i0 < total; i0 += (I)gridDim.x * (TPB * U)) {
+    V w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 + u * TPB < total) w[u] = reinterpret_cast<const V*>(x)[i0 + u * TPB];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 + u * TPB < total) {
+        const I f = (i0 + u * TPB) * VEC;
+        I c, k, b;
+        if (LAST) {
+          I t = f / C;
+          c = f - t * C;
+          if (inner) { const I s = t / Kc; k = t - s * Kc; b = s / HW; }
+          else { const I s = t / HW; k = s / B; b = s - k * B; }
+        } else {
+          const I t = f / HW, s = t / C;
+          c = t - s * C;
+          if (inner) { b = s / Kc; k = s - b * Kc; }
+          else { k = s / B; b = s - k * B; }
+        }
+        const uint32_t uid = (uint32_t)key.uids[k];
+        unsigned m;
+        if (kind == 2) {
+          m = (keep4(key, (uint32_t)(b >> 2), uid, tag) >> (b & 3)) & 1u ? 0xFFu : 0u;
+        } else if (LAST && VEC > 1) {  // channels c .. c + VEC - 1: C and so b * C + c are multiples of VEC
+          const long e = (long)b * C + c;
+          m = keep4(key, (uint32_t)(e >> 2), uid, tag);
+          if (VEC == 8) m |= keep4(key, (uint32_t)(e >> 2) + 1, uid, tag) << 4;
+        } else {
+          const long e = (long)b * C + c;
+          m = (keep4(key, (uint32_t)(e >> 2), uid, tag) >> (e & 3)) & 1u ? 0xFFu : 0u;
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) from_f(to_f(w[u].e[j]) * ((m >> j) & 1u ? key.scale : 0.f), w[u].e[j]);
+        reinterpret_cast<V*>(y)[i0 + u * TPB] = w[u];
+      }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// A draw for every element of channels-last maps: value (b * C + c) * HW + p is counted pixels first, memory runs over
+// channels first.  The draws of CT channels x PT pixels go to LDS, one byte per draw of four in the order they are counted
+// in, then the tile is walked in memory order, VEC channels a thread; its first U vectors are on their way meanwhile.
 constexpr int TILE_BYTES = 8192;
 template <typename T, int VEC>
 __global__ __launch_bounds__(TPB) void drop_last_kernel(Key key, const T* __restrict__ x, T* __restrict__ y, int Kc, int B, int C,
-                                                        int HW, int inner, int kind, int CT, int PT, int ct_n, int pt_n) {
+                                                        int HW, int inner, int CT, int PT, int ct_n, int pt_n) {
   typedef Pack<T, VEC> V;
+  constexpr int U = 4;
   __shared__ unsigned char bits[TILE_BYTES];
   const uint32_t tag = tag_of(key);
   for (long tile = blockIdx.x; tile < (long)Kc * B * ct_n * pt_n; tile += gridDim.x) {
@@ -109,65 +162,74 @@ __global__ __launch_bounds__(TPB) void drop_last_kernel(Key key, const T* __rest
     const uint32_t uid = (uint32_t)key.uids[k];
     const int c0 = ct * CT, cn = min(CT, C - c0), p0 = pt * PT, pn = min(PT, HW - p0);
     const long pitch = inner ? (long)Kc * C : C;
-    const size_t base = inner ? ((size_t)b * HW * Kc + k) * C : ((size_t)k * B + b) * HW * C;
+    const size_t base = (inner ? ((size_t)b * HW * Kc + k) * C : ((size_t)k * B + b) * HW * C) + (size_t)p0 * pitch + c0;
+    const int nvec = cn / VEC, items = nvec * pn;
+    V w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = threadIdx.x + u * TPB, p = i / nvec;
+      if (i < items) w[u] = *reinterpret_cast<const V*>(x + base + (size_t)p * pitch + (i - p * nvec) * VEC);
+    }
     const int nb = (PT + 3) / 4 + 1;  // bytes of a channel
-    if (kind == 0) {
-      for (int i = threadIdx.x; i < cn * nb; i += TPB) {
-        const int c = i / nb, o = i - c * nb;
-        const long s = ((long)b * C + c0 + c) * HW + p0;
-        if (o <= ((s + pn - 1) >> 2) - (s >> 2)) bits[i] = (unsigned char)keep4(key, (uint32_t)((s >> 2) + o), uid, tag);
-      }
-    } else if (kind == 1) {
-      const long s = (long)b * C + c0;
-      for (int i = threadIdx.x; i <= ((s + cn - 1) >> 2) - (s >> 2); i += TPB)
-        bits[i] = (unsigned char)keep4(key, (uint32_t)((s >> 2) + i), uid, tag);
-    } else if (threadIdx.x == 0) {
-      bits[0] = (unsigned char)keep4(key, (uint32_t)(b >> 2), uid, tag);
+    for (int i = threadIdx.x; i < cn * nb; i += TPB) {
+      const int c = i / nb, o = i - c * nb;
+      const long s = ((long)b * C + c0 + c) * HW + p0;
+      if (o <= ((s + pn - 1) >> 2) - (s >> 2)) bits[i] = (unsigned char)keep4(key, (uint32_t)((s >> 2) + o), uid, tag);
     }
     __syncthreads();
-    const int nvec = cn / VEC;
-    for (int i = threadIdx.x; i < nvec * pn; i += TPB) {
+    const int s0 = (int)((((long)b * C + c0) * HW + p0) & 3), sc = HW & 3;
+    auto finish = [&](V v, int i) {
       const int p = i / nvec, c = (i - p * nvec) * VEC;
-      const size_t o = base + (size_t)(p0 + p) * pitch + c0 + c;
-      V w = *reinterpret_cast<const V*>(x + o);
-  #pragma unroll
+#pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        int at, bit;
-        if (kind == 0) {
-          const int s = (int)((((long)b * C + c0 + c + j) * HW + p0) & 3) + p;
-          at = (c + j) * nb + (s >> 2); bit = s & 3;
-        } else if (kind == 1) {
-          const int s = (int)(((long)b * C + c0) & 3) + c + j;
-          at = s >> 2; bit = s & 3;
-        } else {
-          at = 0; bit = b & 3;
-        }
-        from_f(to_f(w.e[j]) * ((bits[at] >> bit) & 1 ? key.scale : 0.f), w.e[j]);
+        const int s = ((s0 + (c + j) * sc) & 3) + p;
+        from_f(to_f(v.e[j]) * ((bits[(c + j) * nb + (s >> 2)] >> (s & 3)) & 1 ? key.scale : 0.f), v.e[j]);
       }
-      *reinterpret_cast<V*>(y + o) = w;
+      *reinterpret_cast<V*>(y + base + (size_t)p * pitch + c) = v;
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if ((int)threadIdx.x + u * TPB < items) finish(w[u], threadIdx.x + u * TPB);
+    for (int i = threadIdx.x + U * TPB; i < items; i += TPB) {
+      const int p = i / nvec;
+      finish(*reinterpret_cast<const V*>(x + base + (size_t)p * pitch + (i - p * nvec) * VEC), i);
     }
     __syncthreads();  // the next tile's draws overwrite these
   }
 }
 
 template <typename T>
-int flat_t(const Key& key, const void* x, void* y, long nblk, int Kc, int inner, long len, long seg, int vec, hipStream_t st) {
-  constexpr int W = 16 / sizeof(T);
-  const long items = seg > 1 || vec > 1 ? len / (vec > 1 ? W : 1) : len / 4 + 2;
-  long gy = nblk < 65535 ? nblk : 65535;
-  long gx = (items + TPB - 1) / TPB, most = 256 * 16 / gy + 1;
+int elem_t(const Key& key, const void* x, void* y, long nblk, int Kc, int inner, long len, int vec, hipStream_t st) {
+  constexpr int W = 16 / sizeof(T), U = 16 / W;  // 16 elements a thread and round
+  const long items = vec ? (len / W + U - 1) / U : len / 4 + 2;
+  const long gy = nblk < 65535 ? nblk : 65535, most = 256 * 16 / gy + 1;
+  long gx = (items + TPB - 1) / TPB;
   if (gx > most) gx = most;
   const dim3 grid((unsigned)gx, (unsigned)gy), block(TPB);
-#define DROP(V, S)                                                                                                     \
-  hipLaunchKernelGGL((drop_flat_kernel<T, V, S>), grid, block, 0, st, key, (const T*)x, (T*)y, nblk, Kc, inner, len, seg)
-  if (seg > 1) { if (vec > 1) DROP(W, true); else DROP(1, true); }
-  else { if (vec > 1) DROP(W, false); else DROP(1, false); }
-#undef DROP
+  if (vec)
+    hipLaunchKernelGGL((drop_elem_kernel<T, W, U>), grid, block, 0, st, key, (const T*)x, (T*)y, nblk, Kc, inner, len);
+  else
+    hipLaunchKernelGGL((drop_elem_kernel<T, 1, 1>), grid, block, 0, st, key, (const T*)x, (T*)y, nblk, Kc, inner, len);
+  return 0;
+}
+
+template <typename T, int VEC, bool LAST>
+int group_v(const Key& key, const void* x, void* y, int Kc, long B, long C, long HW, int inner, int kind, hipStream_t st) {
+  const long elems = Kc * B * C * HW, total = elems / VEC;
+  long gx = (total + 2 * TPB - 1) / (2 * TPB);
+  if (gx > 8192) gx = 8192;
+  const dim3 grid((unsigned)gx), block(TPB);
+  if (elems < (1L << 31))  // (a stride of the grid beyond the end still fits 32 bits)
+    hipLaunchKernelGGL((drop_group_kernel<T, VEC, LAST, uint32_t>), grid, block, 0, st, key, (const T*)x, (T*)y, Kc, (uint32_t)B,
+                       (uint32_t)C, (uint32_t)HW, inner, kind, (uint32_t)total);
+  else
+    hipLaunchKernelGGL((drop_group_kernel<T, VEC, LAST, long>), grid, block, 0, st, key, (const T*)x, (T*)y, Kc, B, C, HW, inner,
+                       kind, total);
   return 0;
 }
 
 template <typename T>
-int last_t(const Key& key, const void* x, void* y, int Kc, int B, int C, int HW, int inner, int kind, int vec, hipStream_t st) {
+int last_t(const Key& key, const void* x, void* y, int Kc, int B, int C, int HW, int inner, int vec, hipStream_t st) {
   constexpr int W = 16 / sizeof(T);
   const int CT = C < 64 ? C : 64;
   int PT = 4 * (TILE_BYTES / CT - 1);  // CT * ((PT + 3) / 4 + 1) <= TILE_BYTES
@@ -178,13 +240,31 @@ int last_t(const Key& key, const void* x, void* y, int Kc, int B, int C, int HW,
   long tiles = (long)Kc * B * ct_n * pt_n;
   if (tiles > (1L << 20)) tiles = 1L << 20;
   const dim3 grid((unsigned)tiles), block(TPB);
-  if (vec > 1)
-    hipLaunchKernelGGL((drop_last_kernel<T, W>), grid, block, 0, st, key, (const T*)x, (T*)y, Kc, B, C, HW, inner, kind, CT, PT,
-                       ct_n, pt_n);
+  if (vec)
+    hipLaunchKernelGGL((drop_last_kernel<T, W>), grid, block, 0, st, key, (const T*)x, (T*)y, Kc, B, C, HW, inner, CT, PT, ct_n,
+                       pt_n);
   else
-    hipLaunchKernelGGL((drop_last_kernel<T, 1>), grid, block, 0, st, key, (const T*)x, (T*)y, Kc, B, C, HW, inner, kind, CT, PT,
-                       ct_n, pt_n);
+    hipLaunchKernelGGL((drop_last_kernel<T, 1>), grid, block, 0, st, key, (const T*)x, (T*)y, Kc, B, C, HW, inner, CT, PT, ct_n,
+                       pt_n);
   return 0;
+}
+
+template <typename T>
+int dropout_t(const Key& key, const void* x, void* y, int Kc, long B, long C, long HW, int kind, int inner, int last, int vec,
+              hipStream_t st) {
+  constexpr int W = 16 / sizeof(T);
+  if (kind == 0) {
+    if (last && HW > 1) return last_t<T>(key, x, y, Kc, (int)B, (int)C, (int)HW, inner, vec && C % W == 0, st);
+    const long nblk = inner ? Kc * B : Kc, len = inner ? C * HW : B * C * HW;
+    return elem_t<T>(key, x, y, nblk, Kc, inner, len, vec && len % W == 0, st);
+  }
+  if (last) {
+    if (vec && C % W == 0) return group_v<T, W, true>(key, x, y, Kc, B, C, HW, inner, kind, st);
+    return group_v<T, 1, true>(key, x, y, Kc, B, C, HW, inner, kind, st);
+  }
+  if (kind == 2) { HW *= C; C = 1; }  // (a sample is one run of memory)
+  if (vec && HW % W == 0) return group_v<T, W, false>(key, x, y, Kc, B, C, HW, inner, kind, st);
+  return group_v<T, 1, false>(key, x, y, Kc, B, C, HW, inner, kind, st);
 }
 }  // namespace
 
@@ -197,18 +277,8 @@ BLADES_API int blades_client_dropout(const void* x, void* y, const long* uids, c
   if (Kc < 1 || B < 1 || C < 1 || HW < 1 || kind < 0 || kind > 2 || dtype < 0 || dtype > 2) return 1;
   if ((double)B * C * HW > 1.7e10) return 1;  // draws of four are counted in 32 bits
   const Key key{uids, tag, tag_value, c3, (uint32_t)seed, (uint32_t)(seed >> 32), least, scale};
-  const int W = dtype == 0 ? 4 : 8;
-  if (last && HW > 1) {
-    if (C > (1 << 30) || HW > (1 << 30) || B > (1 << 30)) return 1;
-    const int v = vec && C % W == 0 ? W : 1;
-    if (dtype == 0) return last_t<float>(key, x, y, Kc, (int)B, (int)C, (int)HW, inner, kind, v, st);
-    if (dtype == 1) return last_t<Bf16>(key, x, y, Kc, (int)B, (int)C, (int)HW, inner, kind, v, st);
-    return last_t<Half>(key, x, y, Kc, (int)B, (int)C, (int)HW, inner, kind, v, st);
-  }
-  const long one = C * HW, seg = kind == 0 ? 1 : kind == 1 ? HW : one;
-  const long nblk = inner ? Kc * B : Kc, len = inner ? one : B * one;
-  const int v = vec && (seg == 1 ? len : seg) % W == 0 && len % W == 0 ? W : 1;
-  if (dtype == 0) return flat_t<float>(key, x, y, nblk, Kc, inner, len, seg, v, st);
-  if (dtype == 1) return flat_t<Bf16>(key, x, y, nblk, Kc, inner, len, seg, v, st);
-  return flat_t<Half>(key, x, y, nblk, Kc, inner, len, seg, v, st);
+  if (C > (1 << 30) || HW > (1 << 30) || B > (1 << 30)) return 1;
+  if (dtype == 0) return dropout_t<float>(key, x, y, Kc, B, C, HW, kind, inner, last, vec, st);
+  if (dtype == 1) return dropout_t<Bf16>(key, x, y, Kc, B, C, HW, kind, inner, last, vec, st);
+  return dropout_t<Half>(key, x, y, Kc, B, C, HW, kind, inner, last, vec, st);
 }

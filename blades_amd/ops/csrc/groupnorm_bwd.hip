@@ -1,0 +1,355 @@
+// Backward pass of the group normalisation: see groupnorm.h.
+#include "groupnorm.h"
+
+namespace {
+using namespace groupnorm;
+
+// g of one vector: gy behind the activation.  The gate byte or z, computed again, decides; z takes the residual again
+// where the activation is smooth.
+template <typename T, int VEC, int AK>
+__device__ __forceinline__ void slope_vector(const Pack<T, VEC>& gy, const float (&xh)[VEC], size_t o, const T* res,
+                                             const unsigned char* gate, const float (&ga)[VEC], const float (&be)[VEC], int act,
+                                             float (&g)[VEC]) {
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) g[j] = to_f(gy.e[j]);
+  if (AK <= 0) {
+    if (act == 0) return;
+  }
+  if (AK <= 0 && gate != nullptr) {
+    const unsigned m = gate[o / VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) g[j] = (m >> j) & 1u ? g[j] : 0.f;
+    return;
+  }
+  float z[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) z[j] = fmaf(xh[j], ga[j], be[j]);
+  if (AK != 0 && res != nullptr) {
+    const Pack<T, VEC> rv = *reinterpret_cast<const Pack<T, VEC>*>(res + o);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) z[j] += to_f(rv.e[j]);
+  }
+  if (AK == 0 || (AK < 0 && act == 1)) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) g[j] = z[j] > 0.f ? g[j] : 0.f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) g[j] *= act_slope<AK>(z[j], act);
+  }
+}
+
+template <typename T, int VEC, int NM>
+__device__ __forceinline__ void bwd_vector(const float (&g)[VEC], const float (&xh)[VEC], size_t o, T* dx, T* dres,
+                                           const float (&rs)[NM], const float (&ga)[VEC], const float (&m1)[NM],
+                                           const float (&m2)[NM]) {
+  typedef Pack<T, VEC> V;
+  if (dx != nullptr) {
+    V w;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const int m = NM == 1 ? 0 : j;
+      from_f(rs[m] * (fmaf(g[j], ga[j], -m1[m]) - xh[j] * m2[m]), w.e[j]);
+    }
+    *reinterpret_cast<V*>(dx + o) = w;
+  }
+  if (dres != nullptr) {
+    V w;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) from_f(g[j], w.e[j]);
+    *reinterpret_cast<V*>(dres + o) = w;
+  }
+}
+
+// Whole samples.  sums [N][C]: (A, B) of every sample and channel.
+template <typename T, int VEC, int R, int NM, int AK>
+__global__ __launch_bounds__(MAX_THREADS) void gn_bwd_kernel(Geo q, const T* __restrict__ x, const T* __restrict__ res,
+                                                                    const T* __restrict__ gy,
+                                                                    const unsigned char* __restrict__ gate,
+                                                                    const float* __restrict__ gamma,
+                                                                    const float* __restrict__ beta,
+                                                                    const float* __restrict__ mean,
+                                                                    const float* __restrict__ rstd, T* __restrict__ dx,
+                                                                    T* __restrict__ dres, float2* __restrict__ sums) {
+  extern __shared__ float lds[];
+  typedef Pack<T, VEC> V;
+  const Place<VEC, NM> w(q);
+  if (!w.here) return;
+  V xr[R], gr[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (w.active && w.row + i * q.rows < w.pn) {
+      xr[i] = *reinterpret_cast<const V*>(x + w.at + i * w.step);
+      gr[i] = *reinterpret_cast<const V*>(gy + w.at + i * w.step);
+    }
+  float *ch = lds, *gam = ch + 2 * q.S, *stat = gam + q.S, *gsum = stat + 2 * w.Gs, *red = gsum + 2 * w.Gs;
+  for (int c = threadIdx.x; c < q.S; c += blockDim.x)
+    gam[c] = gamma ? gamma[w.client * q.gstride + w.slab * q.S + c] : 1.f;
+  for (int g = threadIdx.x; g < w.Gs; g += blockDim.x) {
+    const size_t o = (size_t)w.n * w.G + w.slab * w.Gs + g;
+    stat[g] = mean[o]; stat[w.Gs + g] = rstd[o];
+  }
+  float mu[NM], rs[NM], m1[NM], m2[NM], ga[VEC], be[VEC];
+  if (w.active) load_floats<VEC>(beta ? beta + w.client * q.bstride + w.c0 : nullptr, 0.f, be);
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < NM; ++j) {
+    mu[j] = w.active ? stat[w.g[j]] : 0.f;
+    rs[j] = w.active ? stat[w.Gs + w.g[j]] : 0.f;
+  }
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) ga[j] = w.active ? gam[w.l * VEC + j] : 0.f;
+  float v[2][VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) v[0][j] = v[1][j] = 0.f;
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (w.active && w.row + i * q.rows < w.pn) {
+      float g[VEC], xh[VEC];
+      normed<T, VEC, NM>(xr[i], mu, rs, xh);
+      slope_vector<T, VEC, AK>(gr[i], xh, w.at + i * w.step, res, gate, ga, be, q.act, g);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        v[0][j] += g[j];
+        v[1][j] = fmaf(g[j], xh[j], v[1][j]);
+      }
+      if (sizeof(T) == 4) {  // (fp32: g replaces gy in its registers; a 16-bit type would round it)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) from_f(g[j], gr[i].e[j]);
+      }
+    }
+  slab_sums<2, VEC>(v, 1, q.S, q.tw_ch, q, w.l, w.row, w.active, red, ch);  // ch[0..S): A, ch[S..2S): B
+  for (int c = threadIdx.x; c < q.S; c += blockDim.x)
+    sums[(size_t)w.n * q.C + w.slab * q.S + c] = make_float2(ch[c], ch[q.S + c]);
+  const int tw = q.tw_gr, e0 = threadIdx.x & (tw - 1);
+  for (int g = threadIdx.x / tw; g < 2 * w.Gs; g += blockDim.x / tw) {
+    const int k = g >= w.Gs, cb = (g - k * w.Gs) * q.D;
+    float a = 0.f;
+    for (int e = e0; e < q.D; e += tw) a = fmaf(gam[cb + e], ch[k * q.S + cb + e], a);
+    for (int o = tw >> 1; o > 0; o >>= 1) a += __shfl_xor(a, o, 64);
+    if (e0 == 0) gsum[g] = a;
+  }
+  __syncthreads();
+  if (!w.active || (dx == nullptr && dres == nullptr)) return;
+  const float inv = 1.f / ((float)q.P * (float)q.D);
+#pragma unroll
+  for (int j = 0; j < NM; ++j) { m1[j] = gsum[w.g[j]] * inv; m2[j] = gsum[w.Gs + w.g[j]] * inv; }
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    if (w.row + i * q.rows < w.pn) {
+      const size_t o = w.at + i * w.step;
+      float g[VEC], xh[VEC];
+      normed<T, VEC, NM>(xr[i], mu, rs, xh);
+      if (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) g[j] = to_f(gr[i].e[j]);
+      } else {
+        slope_vector<T, VEC, AK>(gr[i], xh, o, res, gate, ga, be, q.act, g);
+      }
+      bwd_vector<T, VEC, NM>(g, xh, o, dx, dres, rs, ga, m1, m2);
+    }
+}
+
+// Pixel chunks.  APPLY false: part [N][nchunk][C], (A, B) of a chunk.  true: the second sweep, with the joined means [N][G].
+template <typename T, int VEC, int NM, int AK, bool APPLY>
+__global__ __launch_bounds__(MAX_THREADS) void gn_bwd_chunk_kernel(Geo q, const T* __restrict__ x, const T* __restrict__ res,
+                                                           const T* __restrict__ gy, const unsigned char* __restrict__ gate,
+                                                           const float* __restrict__ gamma, const float* __restrict__ beta,
+                                                           const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                           T* __restrict__ dx, T* __restrict__ dres, float2* __restrict__ part,
+                                                           const float2* __restrict__ means) {
+  extern __shared__ float lds[];
+  typedef Pack<T, VEC> V;
+  const Place<VEC, NM> w(q);
+  if (!w.here) return;
+  float mu[NM], rs[NM], m1[NM], m2[NM], ga[VEC], be[VEC], v[2][VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) v[0][j] = v[1][j] = 0.f;
+  if (w.active) {
+#pragma unroll
+    for (int j = 0; j < NM; ++j) {
+      const size_t o = (size_t)w.n * w.G + w.slab * w.Gs + w.g[j];
+      mu[j] = mean[o]; rs[j] = rstd[o];
+      if (APPLY) { const float2 m = means[o]; m1[j] = m.x; m2[j] = m.y; }
+    }
+    load_floats<VEC>(gamma ? gamma + w.client * q.gstride + w.c0 : nullptr, 1.f, ga);
+    load_floats<VEC>(beta ? beta + w.client * q.bstride + w.c0 : nullptr, 0.f, be);
+    for (int p = w.row; p < w.pn; p += BLOCK * q.rows) {
+      V xr[BLOCK], gr[BLOCK];
+      const size_t o = w.at + (size_t)(p - w.row) * q.C;
+#pragma unroll
+      for (int i = 0; i < BLOCK; ++i)
+        if (p + i * q.rows < w.pn) {
+          xr[i] = *reinterpret_cast<const V*>(x + o + i * w.step);
+          gr[i] = *reinterpret_cast<const V*>(gy + o + i * w.step);
+        }
+#pragma unroll
+      for (int i = 0; i < BLOCK; ++i)
+        if (p + i * q.rows < w.pn) {
+          float g[VEC], xh[VEC];
+          normed<T, VEC, NM>(xr[i], mu, rs, xh);
+          slope_vector<T, VEC, AK>(gr[i], xh, o + i * w.step, res, gate, ga, be, q.act, g);
+          if (APPLY) {
+            bwd_vector<T, VEC, NM>(g, xh, o + i * w.step, dx, dres, rs, ga, m1, m2);
+          } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+              v[0][j] += g[j];
+              v[1][j] = fmaf(g[j], xh[j], v[1][j]);
+            }
+          }
+        }
+    }
+  }
+  if (APPLY) return;
+  float *ch = lds, *red = ch + 2 * q.S;
+  slab_sums<2, VEC>(v, 1, q.S, q.tw_ch, q, w.l, w.row, w.active, red, ch);
+  for (int c = threadIdx.x; c < q.S; c += blockDim.x)
+    part[((size_t)w.n * q.nchunk + w.chunk) * q.C + w.slab * q.S + c] = make_float2(ch[c], ch[q.S + c]);
+}
+
+// Joins the chunks' (A, B): channel sums of a sample (for the affine gradients) and gamma times them, 16 channels x 16
+// parts of the chunks a workgroup, fixed order; then the group means for the second sweep, one wave per (sample, group).
+constexpr int JOIN_CH = 16, JOIN_PARTS = 16;
+__global__ __launch_bounds__(JOIN_CH * JOIN_PARTS) void gn_bwd_join_kernel(const float2* __restrict__ part, int n0, int C,
+                                                                          int nchunk, float2* __restrict__ sums) {
+  __shared__ double red[JOIN_PARTS][JOIN_CH][2];
+  const int groups = (C + JOIN_CH - 1) / JOIN_CH, i = blockIdx.x / groups;
+  const int cl = threadIdx.x % JOIN_CH, r = threadIdx.x / JOIN_CH, c = (blockIdx.x - i * groups) * JOIN_CH + cl;
+  double a = 0.0, b = 0.0;
+  if (c < C)
+    for (int k = r; k < nchunk; k += JOIN_PARTS) {
+      const float2 e = part[((size_t)i * nchunk + k) * C + c];
+      a += (double)e.x; b += (double)e.y;
+    }
+  red[r][cl][0] = a; red[r][cl][1] = b;
+  __syncthreads();
+  if (r != 0 || c >= C) return;
+#pragma unroll
+  for (int k = 1; k < JOIN_PARTS; ++k) { a += red[k][cl][0]; b += red[k][cl][1]; }
+  sums[(size_t)(n0 + i) * C + c] = make_float2((float)a, (float)b);
+}
+__global__ __launch_bounds__(256) void gn_bwd_means_kernel(const float2* __restrict__ sums, int n0, int cnt, int C, int D, int P,
+                                                           int per_client, const float* __restrict__ gamma, long gstride,
+                                                           float2* __restrict__ means) {
+  const int G = C / D, lane = threadIdx.x & 63;
+  const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= (long)cnt * G) return;
+  const long n = n0 + i / G;
+  const int g = (int)(i % G);
+  double a = 0.0, b = 0.0;
+  for (int c = g * D + lane; c < (g + 1) * D; c += 64) {
+    const float w = gamma ? gamma[(n / per_client) * gstride + c] : 1.f;
+    const float2 e = sums[(size_t)n * C + c];
+    a += (double)w * e.x; b += (double)w * e.y;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); b += __shfl_xor(b, o, 64); }
+  const double inv = 1.0 / ((double)P * D);
+  if (lane == 0) means[(size_t)n * G + g] = make_float2((float)(a * inv), (float)(b * inv));
+}
+
+// dgamma / dbeta of a client: its samples' (A, B), 8 channels x 128 rows of threads a workgroup, fixed order
+constexpr int AFF_CH = 8, AFF_ROWS = 128;
+__global__ __launch_bounds__(AFF_CH * AFF_ROWS) void gn_affine_kernel(const float2* __restrict__ sums, int per_client, int C,
+                                                                      const float* __restrict__ coef, float* __restrict__ dg,
+                                                                      float* __restrict__ db, long ld, int accumulate) {
+  __shared__ double red[AFF_ROWS][AFF_CH][2];
+  const int chl = threadIdx.x % AFF_CH, r0 = threadIdx.x / AFF_CH, groups = (C + AFF_CH - 1) / AFF_CH;
+  const int k = blockIdx.x / groups, ch = (blockIdx.x - k * groups) * AFF_CH + chl;
+  double a = 0.0, b = 0.0;
+  if (ch < C) {
+    const float2* p = sums + (size_t)k * per_client * C + ch;
+#pragma unroll 4
+    for (int r = r0; r < per_client; r += AFF_ROWS) {
+      const float2 e = p[(size_t)r * C];
+      a += (double)e.x; b += (double)e.y;
+    }
+  }
+  red[r0][chl][0] = a; red[r0][chl][1] = b;
+  for (int o = AFF_ROWS / 2; o > 0; o >>= 1) {
+    __syncthreads();
+    if (r0 < o) { red[r0][chl][0] += red[r0 + o][chl][0]; red[r0][chl][1] += red[r0 + o][chl][1]; }
+  }
+  if (r0 != 0 || ch >= C) return;
+  const float s = coef ? coef[k] : 1.f;
+  const float vg = s * (float)red[0][chl][1], vb = s * (float)red[0][chl][0];
+  if (dg != nullptr) { float* p = dg + k * ld + ch; *p = accumulate ? *p + vg : vg; }
+  if (db != nullptr) { float* p = db + k * ld + ch; *p = accumulate ? *p + vb : vb; }
+}
+
+template <typename T, int VEC, int NM, int AK>
+int backward_t(const Plan& pl, const void* x, const void* res, const void* gy, const unsigned char* gate, const float* gamma,
+               const float* beta, const float* mean, const float* rstd, void* dx, void* dres, float* ws, hipStream_t st) {
+  const Geo& q = pl.q;
+  const int G = q.C / q.D, N = q.N;
+  float2* sums = (float2*)ws;              // [N][C]
+  float2* means = sums + (size_t)N * q.C;  // [N][G]               (these two: split plans alone)
+  float2* part = means + (size_t)N * G;    // [piece][nchunk][C]
+  const size_t per = (size_t)q.P * q.C;
+  for (long n0 = 0; n0 < N; n0 += pl.piece) {
+    Geo s = q;
+    s.N = (int)(N - n0 < pl.piece ? N - n0 : pl.piece);
+    s.first = (int)n0;
+    const T *xp = (const T*)x + n0 * per, *gp = (const T*)gy + n0 * per, *rp = res ? (const T*)res + n0 * per : nullptr;
+    const unsigned char* tp = gate ? gate + n0 * per / VEC : nullptr;
+    T *dp = dx ? (T*)dx + n0 * per : nullptr, *ep = dres ? (T*)dres + n0 * per : nullptr;
+    const float *mp = mean + n0 * G, *sp = rstd + n0 * G;
+    const dim3 grid((unsigned)((s.N + 7) / 8 * 8) * q.nslab * q.nchunk), block(pl.threads);
+    if (pl.split) {
+      hipLaunchKernelGGL((gn_bwd_chunk_kernel<T, VEC, NM, AK, false>), grid, block, pl.lds, st, s, xp, rp, gp, tp, gamma, beta, mp,
+                         sp, (T*)nullptr, (T*)nullptr, part, (const float2*)nullptr);
+      hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)s.N * cdiv(q.C, JOIN_CH)), dim3(JOIN_CH * JOIN_PARTS), 0, st,
+                         (const float2*)part, (int)n0, q.C, q.nchunk, sums);
+      if (dx == nullptr && dres == nullptr) continue;
+      hipLaunchKernelGGL(gn_bwd_means_kernel, dim3(cdiv((long)s.N * G, 4)), dim3(256), 0, st, (const float2*)sums, (int)n0, s.N,
+                         q.C, q.D, q.P, q.per_client, gamma, q.gstride, means);
+      s.back = 1;
+      hipLaunchKernelGGL((gn_bwd_chunk_kernel<T, VEC, NM, AK, true>), grid, block, 0, st, s, xp, rp, gp, tp, gamma, beta, mp, sp, dp,
+                         ep, (float2*)nullptr, (const float2*)(means + n0 * G));
+      continue;
+    }
+#define GN_BWD(RR)                                                                                                         \
+  hipLaunchKernelGGL((gn_bwd_kernel<T, VEC, RR, NM, AK>), grid, block, pl.lds, st, s, xp, rp, gp, tp, gamma, beta, mp, sp, dp, \
+                     ep, sums + n0 * q.C)
+    switch (pl.R) {
+      case 1: case 2: case 4: GN_BWD(4); break;
+      case 8: GN_BWD(8); break;
+      default:  // 16-bit types alone
+        if constexpr (sizeof(T) == 2) GN_BWD(16);
+    }
+#undef GN_BWD
+  }
+  return 0;
+}
+
+}  // namespace
+
+// dx / dres may be null.  dgamma / dbeta: rows of `ld` floats per client (an update matrix's rows or a [clients][C]
+// tensor), scaled by coef[client] (null: 1) and added to what is there where `accumulate`; null: not wanted.
+BLADES_API int blades_group_norm_backward(const void* x, const void* res, const void* gy, const void* gate, const float* gamma,
+                                          const float* beta, const float* mean, const float* rstd, long N, long P, int C,
+                                          int G, int act, int per_client, long gstride, long bstride, void* dx, void* dres,
+                                          const float* coef, float* dgamma, float* dbeta, long ld, int accumulate, float* ws,
+                                          int dtype, int vec, hipStream_t st) {
+  Plan pl;
+  if (!valid(N, P, C, G, vec, dtype, per_client) || act < 0 || act > 3) return 1;
+  if (!make_plan(pl, N, P, C, G, dtype == 0 ? 4 : 2, vec, 2, per_client)) return 2;
+  pl.q.eps = 0.f; pl.q.act = act; pl.q.gstride = gstride; pl.q.bstride = bstride;
+  const unsigned char* gt = (const unsigned char*)gate;
+  int rc;
+#define GN_B(T, V, M, K) rc = backward_t<T, V, M, K>(pl, x, res, gy, gt, gamma, beta, mean, rstd, dx, dres, ws, st)
+#define GN_BT(T)                                                                                  \
+  if (vec == 1) GN_B(T, 1, 1, -1);                                                                \
+  else if (act < 2) { if (pl.one) GN_B(T, 4, 1, 0); else GN_B(T, 4, 4, 0); }                      \
+  else if (act == 2) { if (pl.one) GN_B(T, 4, 1, 2); else GN_B(T, 4, 4, 2); }                     \
+  else { if (pl.one) GN_B(T, 4, 1, 3); else GN_B(T, 4, 4, 3); }
+  if (dtype == 0) { GN_BT(float) }
+  else if (dtype == 1) { GN_BT(Bf16) }
+  else { GN_BT(Half) }
+#undef GN_BT
+#undef GN_B
+  if (rc == 0 && (dgamma != nullptr || dbeta != nullptr))
+    hipLaunchKernelGGL(gn_affine_kernel, dim3((unsigned)(N / per_client) * cdiv(C, AFF_CH)), dim3(AFF_CH * AFF_ROWS), 0, st,
+                       (const float2*)ws, per_client, C, coef, dgamma, dbeta, ld, accumulate);
+  return rc;
+}

@@ -51,45 +51,60 @@ __device__ __forceinline__ void sincos_turns(double turns, float& s, float& c) {
   c = (k == 1 || k == 2) ? -v : v;
 }
 
+// gridDim.y workgroups share a token's S * H rows (`per` each) where there are few tokens.
 template <typename T, int VEC>
-__global__ __launch_bounds__(TPB) void rope_kernel(Freq f, Shape q, const T* x, const void* __restrict__ pos, T* y) {
+__global__ __launch_bounds__(TPB) void rope_kernel(Freq f, Shape q, int per, const T* x, const void* __restrict__ pos, T* y) {
   typedef Pack<T, VEC> V;
+  constexpr int U = 4;
   const int L = q.D / VEC;  // threads of a token
+  const int r0 = blockIdx.y * per, r1 = min(r0 + per, q.slots * q.H);
+  const bool turns = r0 < q.rot * q.H;
+  const bool same = (const void*)x == (const void*)y;
   for (long i = (long)blockIdx.x * TPB + threadIdx.x; i < q.R * q.N * L; i += (long)gridDim.x * TPB) {
     const long token = i / L;
     const int l = (int)(i - token * L);
     const long r = token / q.N, n = token - r * q.N;
-    float sn[VEC / 2], cs[VEC / 2];
-  #pragma unroll
-    for (int j = 0; j < VEC / 2; ++j) {
-      const int pair = l * (VEC / 2) + j, a = f.axis[pair];
-      sn[j] = 0.f; cs[j] = 1.f;
-      if (a != 255) {
-        const long o = r * q.psr + n * q.A + a;
-        const double p = q.pos_float ? (double)static_cast<const float*>(pos)[o] : (double)static_cast<const long*>(pos)[o];
-        sincos_turns(p * f.turns[pair], sn[j], cs[j]);
-        if (q.inverse) sn[j] = -sn[j];
-      }
-    }
     const long xo = r * q.sr + n * q.sn + l * VEC;
     const size_t yo = (size_t)token * q.S * q.H * q.D + (size_t)l * VEC;
-    const bool same = (const void*)x == (const void*)y;
-    for (int s = 0; s < q.slots; ++s) {
-      const bool turn = s < q.rot;
-  #pragma unroll 4
-      for (int h = 0; h < q.H; ++h) {
-        const long at = xo + s * q.ss + h * q.sh;
-        V w = *reinterpret_cast<const V*>(x + at);
-        if (turn) {
-  #pragma unroll
-          for (int j = 0; j < VEC / 2; ++j) {
-            const float a = to_f(w.e[2 * j]), b = to_f(w.e[2 * j + 1]);
-            from_f(fmaf(a, cs[j], -b * sn[j]), w.e[2 * j]);
-            from_f(fmaf(a, sn[j], b * cs[j]), w.e[2 * j + 1]);
-          }
+    float sn[VEC / 2], cs[VEC / 2];
+    if (turns) {
+#pragma unroll
+      for (int j = 0; j < VEC / 2; ++j) {
+        const int pair = l * (VEC / 2) + j, a = f.axis[pair];
+        sn[j] = 0.f; cs[j] = 1.f;
+        if (a != 255) {
+          const long o = r * q.psr + n * q.A + a;
+          const double p = q.pos_float ? (double)static_cast<const float*>(pos)[o] : (double)static_cast<const long*>(pos)[o];
+          sincos_turns(p * f.turns[pair], sn[j], cs[j]);
+          if (q.inverse) sn[j] = -sn[j];
         }
-        *reinterpret_cast<V*>(y + (same ? (size_t)at : yo + ((size_t)s * q.H + h) * q.D)) = w;
       }
+    }
+    int s = r0 / q.H, h = r0 - s * q.H;
+    for (int row = r0; row < r1; row += U) {
+      V w[U];
+      long at[U];
+      bool turn[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        at[u] = xo + s * q.ss + h * q.sh;
+        turn[u] = s < q.rot;
+        if (row + u < r1) w[u] = *reinterpret_cast<const V*>(x + at[u]);
+        if (++h == q.H) { h = 0; ++s; }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (row + u < r1) {
+          if (turn[u]) {
+#pragma unroll
+            for (int j = 0; j < VEC / 2; ++j) {
+              const float a = to_f(w[u].e[2 * j]), b = to_f(w[u].e[2 * j + 1]);
+              from_f(fmaf(a, cs[j], -b * sn[j]), w[u].e[2 * j]);
+              from_f(fmaf(a, sn[j], b * cs[j]), w[u].e[2 * j + 1]);
+            }
+          }
+          *reinterpret_cast<V*>(y + (same ? (size_t)at[u] : yo + (size_t)(row + u) * q.D)) = w[u];
+        }
     }
   }
 }
@@ -115,8 +130,13 @@ BLADES_API int blades_rope_axes(const void* x, void* y, const void* pos, int pos
   const Shape q{R, N, sr, sn, ss, sh, S, H, D, A, rot, x == y ? rot : S, psr, pos_float, inverse};
   long blocks = (R * N * (D / vec) + TPB - 1) / TPB;
   if (blocks > (1L << 20)) blocks = 1L << 20;
-  const dim3 grid((unsigned)blocks), block(TPB);
-#define ROPE(T, V) hipLaunchKernelGGL((rope_kernel<T, V>), grid, block, 0, st, f, q, (const T*)x, pos, (T*)y)
+  // a thread's rows: all of its token, fewer (at least 4 at a time) while the chip's 256 x 8 workgroups are not there
+  const int rows = q.slots * H;
+  if (rows == 0) return 0;
+  int per = rows;
+  while (per > 4 && blocks * ((rows + per - 1) / per) < 2048) per = (per + 1) / 2;
+  const dim3 grid((unsigned)blocks, (unsigned)((rows + per - 1) / per)), block(TPB);
+#define ROPE(T, V) hipLaunchKernelGGL((rope_kernel<T, V>), grid, block, 0, st, f, q, per, (const T*)x, pos, (T*)y)
   if (dtype == 0) { if (vec == 4) ROPE(float, 4); else ROPE(float, 2); }
   else if (dtype == 1) { if (vec == 8) ROPE(Bf16, 8); else ROPE(Bf16, 2); }
   else { if (vec == 8) ROPE(Half, 8); else ROPE(Half, 2); }

@@ -19,12 +19,14 @@ from . import reference as ref
 
 _ACTS = ("none", "relu", "gelu", "silu")
 _KINDS = ("elem", "channel", "sample")
+_POS = (torch.int64, torch.float32)
+_wrapped = torch._C._functorch.is_functorch_wrapped_tensor
 
 
 def _own_kernel(t: torch.Tensor) -> bool:
     from blades_amd import ops
 
-    return t.is_cuda and not ops._FORCE_REFERENCE and not torch._C._functorch.is_functorch_wrapped_tensor(t)
+    return t.is_cuda and not ops._FORCE_REFERENCE and not _wrapped(t)
 
 
 def _h():
@@ -33,42 +35,71 @@ def _h():
     return ops._h()
 
 
+def _kernel_dtype(name, x):
+    if x.dtype not in _h()._DT_CODE:
+        raise ValueError(f"{name}: CUDA tensors must be fp32, bf16 or fp16, got {x.dtype}")
+
+
+def _first_order(backward):
+    """A backward that must not be differentiated again.  torch's wrapper for that costs 6 us a call; it is only needed
+    while a graph of the backward pass is being built."""
+    guarded = once_differentiable(backward)
+
+    def call(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return call
+
+
 class _GroupNormFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, groups, eps, act):
-        h = _h()
-        ctx.lead = [None if t is None else (t.dtype, t.dim()) for t in (weight, bias)]
-        w, b = (None if t is None else t.detach().to(torch.float32) for t in (weight, bias))
-        w, b = (t if t is None or t.stride(-1) == 1 else t.contiguous() for t in (w, b))
-        clients = next((t.shape[0] for t in (w, b) if t is not None and t.dim() == 2), 1)
-        grad = any(ctx.needs_input_grad)
-        y, stats, gate = h.group_norm_forward(x, groups, w, b, eps, act, residual, clients, want_gate=grad)
-        # the gate stands in for the residual; without a ReLU or a residual z is computed again from x
-        keep = residual if gate is None and act in ("gelu", "silu") else None
-        ctx.cfg = (groups, act, clients, gate[1] if gate is not None else 0)
-        ctx.has_res = residual is not None
-        ctx.save_for_backward(x, w, b, stats, keep, gate[0] if gate is not None else None)
+    def forward(ctx, x, weight, bias, residual, cfg):
+        groups, eps, act = cfg
+        w, b = _affine(weight), _affine(bias)
+        clients = _clients(w, b)
+        y, stats, gate = _h().group_norm_forward(x, groups, w, b, eps, act, residual, clients, True, True)
+        # the gate stands in for the residual; without one z is computed again, from x and a smooth activation's residual
+        ctx.cfg = (groups, act, clients, 0 if gate is None else gate[1])
+        ctx.save_for_backward(x, w, b, stats, residual if act in ("gelu", "silu") else None,
+                              None if gate is None else gate[0])
+        ctx.lead = (None if weight is None else weight.dtype, None if bias is None else bias.dtype)
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, gy):
         x, w, b, stats, res, gate = ctx.saved_tensors
         groups, act, clients, gvec = ctx.cfg
-        nx, nw, nb, nr = ctx.needs_input_grad[:4]
-        C = x.shape[1]
-        dw = torch.empty(clients, C, device=x.device) if nw else None
-        db = torch.empty(clients, C, device=x.device) if nb else None
-        dx, dres = _h().group_norm_backward(
-            x, gy, groups, w, b, stats, act, res, (gate, gvec) if gate is not None else None, clients, want_dx=nx,
-            want_dres=nr and act != "none", dweight=dw, dbias=db, ld=C)
+        nx, nw, nb, nr, _ = ctx.needs_input_grad
+        dw = torch.empty(clients, x.shape[1], device=x.device) if nw else None
+        db = torch.empty(clients, x.shape[1], device=x.device) if nb else None
+        dx, dres = _h().group_norm_backward(x, gy, groups, w, b, stats, act, res, (gate, gvec) if gvec else None, clients, nx,
+                                            nr and act != "none", dw, db, x.shape[1], None, False, True)
         if nr and act == "none":
             dres = gy
+        if nw:
+            dw = (dw if w.dim() == 2 else dw[0]).to(ctx.lead[0])
+        if nb:
+            db = (db if b.dim() == 2 else db[0]).to(ctx.lead[1])
+        return dx, dw, db, dres, None
 
-        def as_leaf(t, lead):
-            return None if t is None else t.reshape(t.shape if lead[1] == 2 else (C,)).to(lead[0])
 
-        return dx, as_leaf(dw, ctx.lead[0]), as_leaf(db, ctx.lead[1]), dres if nr else None, None, None, None
+def _affine(t):
+    if t is None:
+        return None
+    t = t.detach().to(torch.float32)
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _clients(*affine):
+    for t in affine:
+        if t is not None and t.dim() == 2:
+            return t.shape[0]
+    return 1
+
+
+def _needs_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def group_norm(x, groups: int, weight=None, bias=None, eps: float = 1e-5, act: str = "none", residual=None):
@@ -77,54 +108,59 @@ def group_norm(x, groups: int, weight=None, bias=None, eps: float = 1e-5, act: s
     ``x [N, C, *]``, read channels last (other layouts are copied); ``weight`` / ``bias`` ``[C]``, or ``[K, C]``: one row
     for each of K clients that own N / K consecutive samples (their gradients then come per client).  ``act``: none, relu,
     gelu (erf) or silu.  Statistics, products and sums are 32-bit, the result is rounded once.  A group has at most 2048
-    channels on the GPU (1024 where C or an address rules out 16-byte accesses)."""
+    channels on the GPU (1024 where C or an address rules out accesses of four)."""
     if x.dim() < 2 or not x.is_floating_point():
         raise ValueError(f"group_norm: expected a floating-point tensor [N, C, *], got {x.dtype} {tuple(x.shape)}")
     N, C = x.shape[0], x.shape[1]
-    groups = int(groups)
+    groups, eps = int(groups), float(eps)
     if groups < 1 or C < 1 or C % groups:
         raise ValueError(f"group_norm: {C} channels do not divide into {groups} groups")
     if act not in _ACTS:
         raise ValueError(f"group_norm: act must be one of {_ACTS}, got {act!r}")
     if not eps >= 0.0:
         raise ValueError(f"group_norm: eps must not be negative, got {eps}")
-    rows = set()
-    for name, t in (("weight", weight), ("bias", bias)):
+    for t in (weight, bias):
         if t is None:
             continue
-        if t.dim() not in (1, 2) or t.shape[-1] != C or not t.is_floating_point() or t.device != x.device:
-            raise ValueError(f"group_norm: {name} must be a floating-point [{C}] or [clients, {C}] tensor on {x.device}, got "
-                             f"{t.dtype} {tuple(t.shape)} on {t.device}")
-        rows.add(t.shape[0] if t.dim() == 2 else 0)
-    if len(rows) > 1 or any(k and N % k for k in rows) or (rows and N and 0 in [t.shape[0] for t in (weight, bias)
-                                                                              if t is not None and t.dim() == 2]):
-        raise ValueError(f"group_norm: weight and bias must be shared or both per client, with {N} samples a multiple of the "
-                         f"clients")
+        if t.dim() not in (1, 2) or t.shape[-1] != C or not t.is_floating_point() or t.device != x.device or (
+                t.dim() == 2 and (t.shape[0] < 1 or N % t.shape[0])):
+            raise ValueError(f"group_norm: weight and bias must be floating-point [{C}] or [clients, {C}] tensors on {x.device}, "
+                             f"the clients dividing {N} samples, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if weight is not None and bias is not None and weight.shape != bias.shape:
+        raise ValueError(f"group_norm: weight {tuple(weight.shape)} and bias {tuple(bias.shape)} must be shared or per client "
+                         f"alike")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
         raise ValueError(f"group_norm: residual must match x ({x.dtype} {tuple(x.shape)}), got {residual.dtype} "
-                         f"{tuple(residual.shape)}")
-    if not _own_kernel(x) or x.numel() == 0:
+                         f"{tuple(residual.shape)} on {residual.device}")
+    if not _own_kernel(x):
         return ref.group_norm(x, groups, weight, bias, eps, act, residual)
-    return _GroupNormFn.apply(x, weight, bias, residual, groups, float(eps), act)
+    _kernel_dtype("group_norm", x)
+    if x.numel() == 0:
+        return ref.group_norm(x, groups, weight, bias, eps, act, residual)
+    if _needs_grad(x, weight, bias, residual):
+        return _GroupNormFn.apply(x, weight, bias, residual, (groups, eps, act))
+    w, b = _affine(weight), _affine(bias)
+    return _h().group_norm_forward(x, groups, w, b, eps, act, residual, _clients(w, b), False, True)[0]
 
 
 class _ClientDropoutFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, uids, tag, cfg):
-        ctx.cfg, ctx.int_tag = cfg, not torch.is_tensor(tag)
-        # (saved, so that changing the ids or the tag between the two passes raises instead of redrawing another mask)
-        ctx.save_for_backward(uids, *([] if ctx.int_tag else [tag]))
-        ctx.tag = tag if ctx.int_tag else None
-        seed, layer, p, kind, layout, scale = cfg
-        return _h().client_dropout(x, uids, seed, tag, layer, p, kind, layout, scale)
+        ctx.cfg, ctx.tag = cfg, tag
+        # the ids and the tag are saved, so that changing them between the two passes raises instead of drawing another mask
+        if torch.is_tensor(tag):
+            ctx.save_for_backward(uids, tag)
+            ctx.tag = None
+        else:
+            ctx.save_for_backward(uids)
+        return _h().client_dropout(x, uids, cfg[0], tag, *cfg[1:], True)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, gy):
-        uids = ctx.saved_tensors[0]
-        tag = ctx.tag if ctx.int_tag else ctx.saved_tensors[1]
-        seed, layer, p, kind, layout, scale = ctx.cfg
-        return _h().client_dropout(gy, uids, seed, tag, layer, p, kind, layout, scale), None, None, None
+        uids, *tag = ctx.saved_tensors
+        cfg = ctx.cfg
+        return _h().client_dropout(gy, uids, cfg[0], tag[0] if tag else ctx.tag, *cfg[1:], True), None, None, None
 
 
 def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "elem", layout: str = "major", scale=None):
@@ -140,38 +176,45 @@ def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "e
         raise ValueError(f"client_dropout: expected a floating-point tensor, got {x.dtype} {tuple(x.shape)}")
     if kind not in _KINDS or layout not in ("major", "inner"):
         raise ValueError(f"client_dropout: kind must be one of {_KINDS}, layout major or inner, got {kind!r}, {layout!r}")
-    if not 0.0 <= float(p) < 1.0:
+    p = float(p)
+    if not 0.0 <= p < 1.0:
         raise ValueError(f"client_dropout: need 0 <= p < 1, got {p}")
-    if uids.dtype != torch.int64 or uids.dim() > 1 or uids.numel() < 1 or uids.device != x.device:
+    K, by_value = uids.numel(), not torch.is_tensor(tag)
+    if uids.dtype != torch.int64 or uids.dim() > 1 or K < 1 or uids.device != x.device:
         raise ValueError("client_dropout: uids must be an int64 vector (or scalar) of clients on x's device")
-    if torch.is_tensor(tag) and (tag.dtype != torch.int64 or tag.numel() != 1 or tag.device != x.device):
+    if not by_value and (tag.dtype != torch.int64 or tag.numel() != 1 or tag.device != x.device):
         raise ValueError("client_dropout: tag must be an int or a 1-element int64 tensor on x's device")
-    K = uids.numel()
-    if layout == "inner" and x.dim() < 2:
+    inner = layout == "inner"
+    if inner and x.dim() < 2:
         raise ValueError("client_dropout: layout inner needs [B, K * C, *]")
-    if x.shape[0 if layout == "major" else 1] % K:
+    if x.shape[1 if inner else 0] % K:
         raise ValueError(f"client_dropout: {tuple(x.shape)} does not divide among {K} clients (layout {layout})")
+    if x.numel() == 0:
+        return x.clone()
     if not _own_kernel(x):
-        if x.numel() == 0:
-            return x.clone()
         return ref.client_dropout(x, uids, seed, tag, layer, p, kind, layout, scale)
-    return _ClientDropoutFn.apply(x, uids.reshape(-1).contiguous(), tag,
-                                  (int(seed), int(layer), float(p), kind, layout, None if scale is None else float(scale)))
+    _kernel_dtype("client_dropout", x)
+    cfg = (int(seed), int(layer), p, kind, layout, None if scale is None else float(scale))
+    if uids.dim() == 0 or not uids.is_contiguous():
+        uids = uids.reshape(-1).contiguous()
+    if by_value:
+        tag = int(tag)
+    if x.requires_grad and torch.is_grad_enabled():
+        return _ClientDropoutFn.apply(x, uids, tag, cfg)
+    return _h().client_dropout(x, uids, cfg[0], tag, *cfg[1:], True)
 
 
 class _RopeFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, pos, axes, base, slots):
+    def forward(ctx, x, pos, cfg):
         ctx.save_for_backward(pos)
-        ctx.cfg = (axes, base, slots)
-        return _h().rope_axes(x, pos, axes, base, slots)
+        ctx.cfg = cfg
+        return _h().rope_axes(x, pos, *cfg, False, None, True)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, gy):
-        (pos,) = ctx.saved_tensors
-        axes, base, slots = ctx.cfg
-        return _h().rope_axes(gy, pos, axes, base, slots, inverse=True), None, None, None, None
+        return _h().rope_axes(gy, ctx.saved_tensors[0], *ctx.cfg, True, None, True), None, None
 
 
 def rope_axes(x, pos, axes, base: float = 10000.0, slots=None):
@@ -181,25 +224,28 @@ def rope_axes(x, pos, axes, base: float = 10000.0, slots=None):
     all) are turned and whose others are copied.  ``axes``: even widths of the sections, one per axis, together at most D
     (the rest of the head passes through).  ``pos``: int64 or fp32 positions, ``[N, A]`` shared by the samples or
     ``[R, N, A]``.  Pair (2i, 2i + 1) of a section d wide is turned by ``pos * base ** (-2 i / d)``; angles are 64-bit.
-    D is even, at most 256 on the GPU; at most 8 axes."""
+    D is even, at most 256; at most 8 axes."""
     if x.dim() not in (4, 5) or not x.is_floating_point():
         raise ValueError(f"rope_axes: expected a floating-point [R, N, H, D] or [R, N, S, H, D] tensor, got {x.dtype} "
                          f"{tuple(x.shape)}")
-    axes = tuple(int(a) for a in axes)
+    axes, base = tuple(int(a) for a in axes), float(base)
     D, S = x.shape[-1], x.shape[2] if x.dim() == 5 else 1
     if not axes or len(axes) > 8 or any(a < 2 or a % 2 for a in axes) or sum(axes) > D or D % 2 or D > 256:
         raise ValueError(f"rope_axes: 1 to 8 even sections that fit an even head dimension of at most 256 are needed, got "
                          f"{axes} for {D}")
-    if slots is not None and not 0 <= int(slots) <= S:
-        raise ValueError(f"rope_axes: slots must lie in 0 .. {S}, got {slots}")
-    if not float(base) > 0.0:
-        raise ValueError(f"rope_axes: base must be positive, got {base}")
-    want = (x.shape[1], len(axes))
-    if pos.dtype not in (torch.int64, torch.float32) or tuple(pos.shape) not in (want, (x.shape[0],) + want) \
-            or pos.device != x.device or pos.requires_grad:
-        raise ValueError(f"rope_axes: pos must be int64 or fp32 {list(want)} or {[x.shape[0], *want]} on {x.device} without a "
-                         f"gradient, got {pos.dtype} {tuple(pos.shape)} on {pos.device}")
     slots = S if slots is None else int(slots)
+    if not 0 <= slots <= S:
+        raise ValueError(f"rope_axes: slots must lie in 0 .. {S}, got {slots}")
+    if not 0.0 < base < float("inf"):
+        raise ValueError(f"rope_axes: base must be positive and finite, got {base}")
+    shape = pos.shape
+    if pos.dtype not in _POS or shape[-2:] != (x.shape[1], len(axes)) or len(shape) > 3 or (
+            len(shape) == 3 and shape[0] != x.shape[0]) or pos.device != x.device or pos.requires_grad:
+        raise ValueError(f"rope_axes: pos must be int64 or fp32 [{x.shape[1]}, {len(axes)}] or [{x.shape[0]}, {x.shape[1]}, "
+                         f"{len(axes)}] on {x.device} without a gradient, got {pos.dtype} {tuple(shape)} on {pos.device}")
     if not _own_kernel(x):
-        return ref.rope_axes(x, pos, axes, float(base), slots)
-    return _RopeFn.apply(x, pos, axes, float(base), slots)
+        return ref.rope_axes(x, pos, axes, base, slots)
+    _kernel_dtype("rope_axes", x)
+    if x.requires_grad and torch.is_grad_enabled():
+        return _RopeFn.apply(x, pos, (axes, base, slots))
+    return _h().rope_axes(x, pos, axes, base, slots, False, None, True)
