@@ -111,6 +111,10 @@ def _empty_like(*a, **k):
     return _poison(torch.empty_like(*a, **k))
 
 
+if not _POISON:  # (nothing to fill: the functions themselves, without a call in between)
+    _empty, _empty_like = torch.empty, torch.empty_like
+
+
 def _stream():
     return c_void_p(torch.cuda.current_stream().cuda_stream)
 
@@ -1786,24 +1790,22 @@ def ce_topk(logits, labels, ks):
 # client-keyed dropout without a stored mask (dropout.hip), rotary positions with several axes (rope.hip)
 _DT_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACT_CODE = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
-_gn_ws = _opt_sig("blades_group_norm_ws", [c_long, c_long, c_int, c_int, c_int, c_int, c_int], c_long)
-_gn_fwd = _opt_sig("blades_group_norm_forward", [_P, _P, _P, _P, c_long, c_long, c_int, c_int, c_float, c_int, c_int, c_long,
-                                                 c_long, _P, _P, _P, _P, _P, c_int, c_int, _P], c_int)
-_gn_bwd = _opt_sig("blades_group_norm_backward", [_P, _P, _P, _P, _P, _P, _P, _P, c_long, c_long, c_int, c_int, c_int, c_int,
-                                                  c_long, c_long, _P, _P, _P, _P, _P, c_long, c_int, _P, c_int, c_int, _P],
-                   c_int)
-_client_drop = _opt_sig("blades_client_dropout", [_P, _P, _P, _P, c_long, c_int, c_long, c_long, c_long, c_int, c_int, c_int,
-                                                  c_uint, c_ulonglong, c_uint, c_float, c_int, c_int, _P], c_int)
-_rope = _opt_sig("blades_rope_axes", [_P, _P, _P, c_int, c_long, c_long, c_long, c_int, c_int, c_int, c_long, c_long, c_long,
-                                      c_long, c_int, _P, c_int, c_double, c_int, c_int, c_int, _P], c_int)
+_gn_plan_size = _opt_sig("blades_group_norm_plan_size", [], c_long)
+_gn_plan_fill = _opt_sig("blades_group_norm_plan", [_P, c_long, c_long, c_int, c_int, c_float, c_int, c_int, c_long, c_long,
+                                                    c_int, c_int, _P], c_int)
+_gn_fwd = _opt_sig("blades_group_norm_forward", [_P] * 10, c_int)
+_gn_bwd = _opt_sig("blades_group_norm_backward", [_P] * 12 + [c_long, c_int] + [_P] * 3, c_int)
+_client_drop = _opt_sig("blades_client_dropout", [_P, _P, _P, _P, c_long, _P, _P], c_int)
+_rope_plan_size = _opt_sig("blades_rope_plan_size", [], c_long)
+_rope_plan_fill = _opt_sig("blades_rope_plan", [_P, c_int, c_long, c_long, c_long, c_int, c_int, c_int, c_long, c_long, c_long,
+                                                c_long, c_int, _P, c_int, c_double, c_int, c_int], c_int)
+_rope = _opt_sig("blades_rope_axes", [_P, _P, _P, _P, c_int, _P], c_int)
+_raw_stream, _device_now = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _dp(t):
     """Address of a tensor for a ctypes pointer argument (None: null)."""
     return None if t is None else t.data_ptr()
-
-
-_raw_stream, _device_now = torch._C._cuda_getCurrentRawStream, torch.cuda.current_device
 
 
 def _launch(index: int, fn, *args):
@@ -1834,36 +1836,56 @@ def _like_channels_last(x):
     return _empty([x.shape[0]] + list(x.shape[2:]) + [x.shape[1]], dtype=x.dtype, device=x.device).movedim(-1, 1)
 
 
+class _GnPlan:
+    """Launch plan of both directions of a group norm, a function of sizes alone."""
+
+    __slots__ = ("buf", "at", "ws", "vec")
+
+    def __init__(self, N, P, C, G, eps, act, per_client, gstride, bstride, dt, vec):
+        self.buf = ctypes.create_string_buffer(_gn_plan_size())
+        self.at, self.vec = ctypes.addressof(self.buf), vec
+        ws = (c_long * 2)()
+        rc = _gn_plan_fill(self.at, N, P, C, G, eps, act, per_client, gstride, bstride, dt, vec, ws)
+        if rc == 1:
+            raise ValueError("group_norm: rejected")
+        self.ws = None if rc else (ws[0], ws[1])
+
+
 @functools.lru_cache(maxsize=4096)
-def _gn_plan(N, P, C, G, dt, vec, direction):
-    """(channels per access, workspace bytes) of a shape; workspace -1: not supported."""
-    ws = _gn_ws(N, P, C, G, dt, vec, direction)
-    if ws < 0 and vec > 1:  # wide groups of an odd number of channels
-        vec = 1
-        ws = _gn_ws(N, P, C, G, dt, vec, direction)
-    return vec, ws
+def _gn_plan(N, P, C, G, eps, act, per_client, gstride, bstride, dt, vec):
+    """The plan; fewer channels per access than asked for where groups of an odd number of channels are wide.  ws None: not
+    supported."""
+    plan = _GnPlan(N, P, C, G, eps, act, per_client, gstride, bstride, dt, vec)
+    if plan.ws is None and vec > 1:
+        plan = _GnPlan(N, P, C, G, eps, act, per_client, gstride, bstride, dt, 1)
+    return plan
 
 
-def _gn_layout(x, G, direction, other, residual):
-    """(N, P, C, dtype code, channels per access, workspace bytes): four channels where their count and every address
-    allow them."""
-    N, C = x.shape[0], x.shape[1]
-    P = x.numel() // (N * C)
-    dt = _DT_CODE[x.dtype]
-    a = x.data_ptr() | (0 if other is None else other.data_ptr()) | (0 if residual is None else residual.data_ptr())
-    w = 1 if C % 4 or a % (16 if dt == 0 else 8) else 4
-    vec, ws = _gn_plan(N, P, C, G, dt, w, direction)
-    if ws < 0:
-        raise ValueError(f"group_norm: {C} channels in {G} groups over {P} pixels are not supported (a group has at most 2048 "
-                         f"channels; 1024 where C or an address rules out accesses of four)")
-    return N, P, C, dt, vec, ws
+def group_norm_plan(x, G, eps, act, clients, weight, bias, *others, vec=0):
+    """Plan for channels-last ``x``: four channels per access where their count and every address allow them."""
+    shape = x.shape
+    N, C = shape[0], shape[1]
+    if not vec:
+        a = x.data_ptr()
+        for t in others:
+            if t is not None:
+                a |= t.data_ptr()
+        vec = 1 if C % 4 or a % 16 else 4
+    plan = _gn_plan(N, x.numel() // (N * C), C, G, eps, ACT_CODE[act], N // clients,
+                    0 if weight is None or weight.dim() == 1 else weight.stride(0),
+                    0 if bias is None or bias.dim() == 1 else bias.stride(0), _DT_CODE[x.dtype], vec)
+    if plan.ws is None:
+        raise ValueError(f"group_norm: {C} channels in {G} groups over {x.numel() // (N * C)} pixels are not supported (a group "
+                         f"has at most 2048 channels; 1024 where C or an address rules out accesses of four)")
+    return plan
 
 
 def group_norm_supported(x: torch.Tensor, groups: int) -> bool:
-    if _gn_ws is None or not (x.is_cuda and x.dtype in _DT_CODE and x.dim() >= 2 and x.numel() > 0):
+    if _gn_fwd is None or not (x.is_cuda and x.dtype in _DT_CODE and x.dim() >= 2 and x.numel() > 0):
         return False
     N, C = x.shape[0], x.shape[1]
-    return C % groups == 0 and _gn_plan(N, x.numel() // (N * C), C, groups, _DT_CODE[x.dtype], 1, 1)[1] >= 0
+    return C % groups == 0 and _gn_plan(N, x.numel() // (N * C), C, groups, 1e-5, 0, N, 0, 0, _DT_CODE[x.dtype],
+                                        1).ws is not None
 
 
 def _gn_check(name, x, groups, clients, weight, bias, *others):
@@ -1884,46 +1906,37 @@ def _gn_check(name, x, groups, clients, weight, bias, *others):
                              f"on {x.device}")
 
 
-def _gn_stride(t) -> int:
-    return 0 if t is None or t.dim() == 1 else t.stride(0)
-
-
 def group_norm_forward(x, groups: int, weight, bias, eps: float, act: str = "none", residual=None, clients: int = 1,
                        for_backward: bool = True, checked: bool = False):
     """``act(group_norm(x) * weight + bias + residual)`` for channels-last ``x [N, C, *]`` (fp32, bf16 or fp16).
-    ``weight`` / ``bias``: fp32 ``[C]`` or ``[clients, C]`` (any client stride).  Returns (y, stats, gate).  For a backward
-    pass: stats ``[2, N, groups]`` (mean, 1 / std) and, for a ReLU behind a residual, its gate, one byte per vector, which
-    spares that pass the residual: (bytes, elements per vector); else None.  ``checked``: the caller did."""
+    ``weight`` / ``bias``: fp32 ``[C]`` or ``[clients, C]`` (any client stride).  Returns (y, stats, gate, plan).  For a
+    backward pass: stats ``[2, N, groups]`` (mean, 1 / std) and, for a ReLU behind a residual, its gate, one byte per vector,
+    which spares that pass the residual; else None.  ``checked``: the caller did."""
     if not checked:
         _gn_check("group_norm", x, groups, clients, weight, bias, residual)
     x = to_channels_last(x)
     residual = None if residual is None else to_channels_last(residual)
-    N, P, C, dt, vec, ws_bytes = _gn_layout(x, groups, 0, None, residual)
-    dev = x.device
+    plan = group_norm_plan(x, groups, eps, act, clients, weight, bias, residual)
     y = _like_channels_last(x)
     stats = gate = ws = None
-    mean = rstd = None
-    if for_backward or ws_bytes:
-        stats = _empty(2, N, groups, dtype=torch.float32, device=dev)
-        mean = stats.data_ptr()
-        rstd = mean + 4 * N * groups
+    if for_backward or plan.ws[0]:
+        stats = _empty(2, x.shape[0], groups, dtype=torch.float32, device=x.device)
     if for_backward and residual is not None and act == "relu":
-        gate = _empty(x.numel() // vec, dtype=torch.uint8, device=dev)
-    if ws_bytes:
-        ws = _empty(ws_bytes, dtype=torch.uint8, device=dev)
-    rc = _launch(dev.index, _gn_fwd, x.data_ptr(), _dp(residual), _dp(weight), _dp(bias), N, P, C, groups, eps, ACT_CODE[act],
-                 N // clients, _gn_stride(weight), _gn_stride(bias), y.data_ptr(), _dp(gate), mean, rstd, _dp(ws), dt, vec)
-    if rc != 0:
-        raise ValueError(f"group_norm: rejected (rc={rc})")
-    return y, stats, None if gate is None else (gate, vec)
+        gate = _empty(x.numel() // plan.vec, dtype=torch.uint8, device=x.device)
+    if plan.ws[0]:
+        ws = _empty(plan.ws[0], dtype=torch.uint8, device=x.device)
+    _launch(x.device.index, _gn_fwd, x.data_ptr(), _dp(residual), _dp(weight), _dp(bias), y.data_ptr(), _dp(gate), _dp(stats),
+            _dp(ws), plan.at)
+    return y, stats, gate, plan
 
 
-def group_norm_backward(x, gy, groups: int, weight, bias, stats, act: str = "none", residual=None, gate=None, clients: int = 1,
-                        want_dx: bool = True, want_dres: bool = False, dweight=None, dbias=None, ld: int = 0, coef=None,
-                        accumulate: bool = False, checked: bool = False):
-    """Gradients of ``group_norm_forward``: returns (dx, dres).  ``dweight`` / ``dbias``: fp32 ``[clients, C]`` tensors, rows
-    ``ld`` floats apart (columns of the update matrix, for one); they receive — ``accumulate``: are incremented by —
-    ``coef[client]`` (None: 1) times the sums.  ``gate``: as the forward pass returned it, in place of the residual."""
+def group_norm_backward(x, gy, groups: int, weight, bias, stats, plan, act: str = "none", residual=None, gate=None,
+                        clients: int = 1, want_dx: bool = True, want_dres: bool = False, dweight=None, dbias=None, ld: int = 0,
+                        coef=None, accumulate: bool = False, checked: bool = False):
+    """Gradients of ``group_norm_forward``, whose ``stats``, ``gate`` and ``plan`` these are: returns (dx, dres).
+    ``dweight`` / ``dbias``: fp32 ``[clients, C]`` tensors, rows ``ld`` floats apart (columns of the update matrix, for one);
+    they receive — ``accumulate``: are incremented by — ``coef[client]`` (None: 1) times the sums.  ``gate`` stands in for the
+    residual."""
     if not checked:
         _gn_check("group_norm_backward", x, groups, clients, weight, bias, gy, residual)
         N, C = x.shape[0], x.shape[1]
@@ -1936,28 +1949,21 @@ def group_norm_backward(x, gy, groups: int, weight, bias, stats, act: str = "non
                 raise ValueError(f"group_norm_backward: {n} must be fp32 [{clients}, {C}] with row stride ld")
         if coef is not None:
             coef = _vec(coef, clients, x.device, name="coef")
-        if gate is not None and (gate[0].numel() * gate[1] != x.numel() or gate[0].device != x.device):
+        if gate is not None and (gate.numel() * plan.vec != x.numel() or gate.device != x.device):
             raise ValueError("group_norm_backward: the gate does not match x")
     x, gy = to_channels_last(x), to_channels_last(gy)
     residual = None if residual is None or gate is not None else to_channels_last(residual)
-    N, P, C, dt, vec, ws_bytes = _gn_layout(x, groups, 1, gy, residual)
-    bits = None
-    if gate is not None:
-        bits, gvec = gate
-        if gvec != vec:  # the gate's vectors decide: the two passes saw different alignments
-            if gvec > 1:
-                x, gy = (t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.preserve_format) for t in (x, gy))
-            vec, ws_bytes = _gn_plan(N, P, C, groups, dt, gvec, 1)
-    dev = x.device
+    if plan.vec > 1 and (x.data_ptr() | gy.data_ptr() | (0 if residual is None else residual.data_ptr())) % 16:
+        if gate is None:
+            plan = group_norm_plan(x, groups, 0.0, act, clients, weight, bias, vec=1)
+        else:  # the gate's vectors decide
+            x, gy = (t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.preserve_format) for t in (x, gy))
     dx = _like_channels_last(x) if want_dx else None
     dres = _like_channels_last(x) if want_dres else None
-    ws = _empty(ws_bytes, dtype=torch.uint8, device=dev)
-    mean = stats.data_ptr()
-    rc = _launch(dev.index, _gn_bwd, x.data_ptr(), _dp(residual), gy.data_ptr(), _dp(bits), _dp(weight), _dp(bias), mean,
-                 mean + 4 * N * groups, N, P, C, groups, ACT_CODE[act], N // clients, _gn_stride(weight), _gn_stride(bias),
-                 _dp(dx), _dp(dres), _dp(coef), _dp(dweight), _dp(dbias), ld, int(accumulate), ws.data_ptr(), dt, vec)
-    if rc != 0:
-        raise ValueError(f"group_norm_backward: rejected (rc={rc})")
+    ws = _empty(plan.ws[1], dtype=torch.uint8, device=x.device)
+    _launch(x.device.index, _gn_bwd, x.data_ptr(), _dp(residual), gy.data_ptr(), _dp(gate), _dp(weight), _dp(bias),
+            stats.data_ptr(), _dp(dx), _dp(dres), _dp(coef), _dp(dweight), _dp(dbias), ld, int(accumulate), ws.data_ptr(),
+            plan.at)
     return dx, dres
 
 
@@ -1967,9 +1973,14 @@ def dropout_scale(p: float) -> float:
     return c_float(1.0 / q).value
 
 
+class _DropPlan(ctypes.Structure):
+    _fields_ = [("B", c_long), ("C", c_long), ("HW", c_long), ("seed", c_ulonglong), ("Kc", c_int), ("kind", c_int),
+                ("inner", c_int), ("last", c_int), ("dtype", c_int), ("c3", c_uint), ("least", c_uint), ("scale", c_float)]
+
+
 @functools.lru_cache(maxsize=4096)
-def _drop_plan(shape, Kc, kind, layout, last, layer, seed, p, scale, dt):
-    """The arguments of a client_dropout launch that its shape and key fix."""
+def _drop_plan(shape, Kc, last, dtype, seed, layer, p, kind, layout, scale):
+    """(plan, its address): what a client_dropout launch's shape and key fix."""
     if layout == "major":
         B, C = shape[0] // Kc, (shape[1] if len(shape) > 1 else 1)
     else:
@@ -1977,9 +1988,13 @@ def _drop_plan(shape, Kc, kind, layout, last, layer, seed, p, scale, dt):
     numel = 1
     for d in shape:
         numel *= d
-    code = {"elem": 0, "channel": 1 if len(shape) > 2 else 0, "sample": 2}[kind]
-    return (Kc, B, C, numel // (Kc * B * C), code, int(layout == "inner"), int(last), (2 + 256 * layer) & 0xFFFFFFFF,
-            seed & (2 ** 64 - 1), _ceil(c_float(p).value * 16777216.0), dropout_scale(p) if scale is None else scale, dt)
+    if numel // Kc > 17e9:
+        raise ValueError("client_dropout: a client's share of a layer has at most 1.7e10 elements")
+    plan = _DropPlan(B, C, numel // (Kc * B * C), seed & (2 ** 64 - 1), Kc,
+                     {"elem": 0, "channel": 1 if len(shape) > 2 else 0, "sample": 2}[kind], layout == "inner", last,
+                     _DT_CODE[dtype], (2 + 256 * layer) & 0xFFFFFFFF, _ceil(c_float(p).value * 16777216.0),
+                     dropout_scale(p) if scale is None else scale)
+    return plan, ctypes.addressof(plan)
 
 
 def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "elem", layout: str = "major", scale=None,
@@ -1994,42 +2009,59 @@ def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "e
             raise ValueError("client_dropout: uids must be a contiguous int64 vector on x's device that divides the batch")
         if torch.is_tensor(tag) and not (tag.device == x.device and tag.dtype == torch.int64 and tag.numel() == 1):
             raise ValueError("client_dropout: tag must be an int or a 1-element int64 tensor on x's device")
+        tag = tag if torch.is_tensor(tag) else int(tag)
         if not 0.0 <= p < 1.0:
             raise ValueError("client_dropout: need 0 <= p < 1")
     if x.numel() == 0:
         return x.clone()
+    x, plan = dropout_plan(x, uids, seed, layer, p, kind, layout, scale)
+    return dropout_launch(x, uids, tag, plan)
+
+
+def dropout_plan(x, uids, seed, layer, p, kind, layout, scale):
+    """(x as the kernel takes it, plan)."""
     last = False
     if not x.is_contiguous():
         last = x.dim() == 4 and x.is_contiguous(memory_format=torch.channels_last)
         x = x if last else x.contiguous()
+    return x, _drop_plan(x.shape, uids.numel(), last, x.dtype, seed, layer, p, kind, layout, scale)
+
+
+def dropout_launch(x, uids, tag, plan):
+    """The plan's dropout of a tensor that lies as the one the plan was made for.  ``tag``: int, or tensor."""
     y = _empty_like(x)
-    at, to = x.data_ptr(), y.data_ptr()
-    plan = _drop_plan(tuple(x.shape), uids.numel(), kind, layout, last, layer, seed, p, scale, _DT_CODE[x.dtype])
-    by_value = not torch.is_tensor(tag)
-    rc = _launch(x.device.index, _client_drop, at, to, uids.data_ptr(), None if by_value else tag.data_ptr(),
-                 tag if by_value else 0, *plan, int(at % 16 == 0 and to % 16 == 0))
+    value, at = (tag, None) if type(tag) is int else (0, tag.data_ptr())
+    rc = _launch(x.device.index, _client_drop, x.data_ptr(), y.data_ptr(), uids.data_ptr(), at, value, plan[1])
     if rc != 0:
-        raise ValueError(f"client_dropout: rejected (rc={rc}): a client's share of a layer has at most 1.7e10 elements")
+        raise ValueError(f"client_dropout: rejected (rc={rc})")
     return y
 
 
-@functools.lru_cache(maxsize=1024)
-def _c_ints(values):
-    return (c_int * len(values))(*values)
+@functools.lru_cache(maxsize=4096)
+def _rope_plan(shape, stride, five, per_sample, pos_float, dtype, narrow, axes, base, slots):
+    """(plan, its address): what a rope_axes launch's shape fixes."""
+    R, N, H, D = shape[0], shape[1], shape[-2], shape[-1]
+    dt = _DT_CODE[dtype]
+    plan = ctypes.create_string_buffer(_rope_plan_size())
+    rc = _rope_plan_fill(plan, pos_float, N * len(axes) if per_sample else 0, R, N, shape[2] if five else 1, H, D, stride[0],
+                         stride[1], stride[2] if five else 0, stride[-2], slots, (c_int * len(axes))(*axes), len(axes), base, dt,
+                         2 if narrow else (4 if dt == 0 else 8))
+    if rc != 0:
+        raise ValueError(f"rope_axes: rejected (rc={rc})")
+    return plan, ctypes.addressof(plan)
 
 
 def rope_axes(x, pos, axes, base: float = 10000.0, slots=None, inverse: bool = False, out=None, checked: bool = False):
     """Rotary positions with several axes (see reference.rope_axes).  ``x`` may have any strides (last dimension
     contiguous).  ``out``: None for a new contiguous tensor, or ``x`` itself: turned in place, other slots untouched.
     ``checked``: the caller did, and ``axes`` is a tuple of ints, ``slots`` an int."""
-    five = x.dim() == 5
-    R, N, D = x.shape[0], x.shape[1], x.shape[-1]
-    S, H = (x.shape[2], x.shape[3]) if five else (1, x.shape[2])
+    shape, five = x.shape, x.dim() == 5
     if not checked:
+        R, N, D, S = shape[0], shape[1], shape[-1], shape[2] if five else 1
         axes, slots = tuple(int(a) for a in axes), S if slots is None else int(slots)
         if not (x.is_cuda and x.dtype in _DT_CODE and x.dim() in (4, 5)):
             raise ValueError(f"rope_axes: expected a CUDA fp32 / bf16 / fp16 tensor [R, N, H, D] or [R, N, S, H, D], got "
-                             f"{x.device} {x.dtype} {tuple(x.shape)}")
+                             f"{x.device} {x.dtype} {tuple(shape)}")
         if not axes or len(axes) > 8 or any(a < 2 or a % 2 for a in axes) or sum(axes) > D or D % 2 or D > 256:
             raise ValueError(f"rope_axes: sections {axes} must be even and fit the head dimension {D} (even, at most 256)")
         if not 0 <= slots <= S or not base > 0.0:
@@ -2040,25 +2072,28 @@ def rope_axes(x, pos, axes, base: float = 10000.0, slots=None, inverse: bool = F
                              f"device, got {pos.dtype} {tuple(pos.shape)} on {pos.device}")
         if out is not None and (out is not x or x.stride(-1) != 1 or not _no_overlap(x)):
             raise ValueError("rope_axes: out must be x itself, without overlapping elements, its last dimension contiguous")
-    pos = pos.contiguous()
+    if not pos.is_contiguous():
+        pos = pos.contiguous()
     if x.numel() == 0:
-        return x if out is not None else _empty(x.shape, dtype=x.dtype, device=x.device)
-    if x.stride(-1) != 1:
+        return x if out is not None else _empty(shape, dtype=x.dtype, device=x.device)
+    stride = x.stride()
+    if stride[-1] != 1:
         x = x.contiguous()
-    dt = _DT_CODE[x.dtype]
-    w = 4 if dt == 0 else 8
-    st = x.stride()
-    sr, sn, ss, sh = st[0], st[1], st[2] if five else 0, st[-2]
-    if D % w or (sr | sn | ss | sh) % w or x.data_ptr() % 16:
-        w = 2
-        if (sr | sn | ss | sh) % 2 or x.data_ptr() % (2 * x.element_size()):
+        stride = x.stride()
+    at = x.data_ptr()
+    narrow = False
+    step = stride[0] | stride[1] | stride[2] | stride[-2]
+    w = 16 // x.element_size()
+    if at % 16 or step % w or shape[-1] % w:
+        narrow = True
+        if step % 2 or at % (2 * x.element_size()):
             if out is not None:
                 raise ValueError("rope_axes: in place needs pairs at even addresses")
-            return rope_axes(x.clone(memory_format=torch.contiguous_format), pos, axes, base, slots, inverse, None, True)
-    y = x if out is not None else _empty(x.shape, dtype=x.dtype, device=x.device)
-    rc = _launch(x.device.index, _rope, x.data_ptr(), y.data_ptr(), pos.data_ptr(), int(pos.dtype == torch.float32),
-                 N * len(axes) if pos.dim() == 3 else 0, R, N, S, H, D, sr, sn, ss, sh, slots, _c_ints(axes), len(axes), base,
-                 int(inverse), dt, w)
+            x = x.clone(memory_format=torch.contiguous_format)
+            return rope_axes(x, pos, axes, base, slots, inverse, None, True)
+    plan = _rope_plan(shape, stride, five, pos.dim() == 3, pos.dtype == torch.float32, x.dtype, narrow, axes, base, slots)
+    y = x if out is not None else _empty(shape, dtype=x.dtype, device=x.device)
+    rc = _launch(x.device.index, _rope, at, y.data_ptr(), pos.data_ptr(), plan[1], inverse)
     if rc != 0:
         raise ValueError(f"rope_axes: rejected (rc={rc})")
     return y

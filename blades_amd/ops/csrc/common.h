@@ -33,6 +33,21 @@ __device__ __forceinline__ float block_sum_256(float v, float* red) {
   return red[0] + red[1] + red[2] + red[3];
 }
 
+// A kernel's output, past the caches' replacement where `through` (a uniform value).  What a rule for it has to weigh: the
+// kernel itself does not wait for write-backs, but what reads the output next finds less of it near.
+template <typename V> __device__ __forceinline__ void store_out(void* p, const V& v, bool through) {
+  if constexpr (sizeof(V) % 4 == 0) {
+    typedef unsigned words __attribute__((ext_vector_type(sizeof(V) / 4)));
+    if (through) {
+      asm volatile("");  // (before and after: keeps the compiler from making one plain store of both)
+      __builtin_nontemporal_store(__builtin_bit_cast(words, v), (words*)p);
+      asm volatile("");
+      return;
+    }
+  }
+  *(V*)p = v;
+}
+
 static inline int cdiv(long a, long b) { return (int)((a + b - 1) / b); }
 
 // Philox4x32-10 — bit-identical to ops/reference.py::_philox4x32.

@@ -268,17 +268,28 @@ int dropout_t(const Key& key, const void* x, void* y, int Kc, long B, long C, lo
 }
 }  // namespace
 
-// dtype 0 fp32, 1 bf16, 2 fp16.  kind 0 element, 1 channel, 2 sample.  last: channels-last maps, else contiguous
-// [.., C, HW].  inner: [B][Kc][C] instead of [Kc][B][C] in the leading dimensions.  vec != 0: 16-byte accesses are
-// allowed (the caller checked the addresses; lengths are checked here).  least: smallest 24-bit draw that is kept.
-BLADES_API int blades_client_dropout(const void* x, void* y, const long* uids, const long* tag, long tag_value, int Kc, long B,
-                                     long C, long HW, int kind, int inner, int last, unsigned c3, unsigned long long seed,
-                                     unsigned least, float scale, int dtype, int vec, hipStream_t st) {
-  if (Kc < 1 || B < 1 || C < 1 || HW < 1 || kind < 0 || kind > 2 || dtype < 0 || dtype > 2) return 1;
-  if ((double)B * C * HW > 1.7e10) return 1;  // draws of four are counted in 32 bits
-  const Key key{uids, tag, tag_value, c3, (uint32_t)seed, (uint32_t)(seed >> 32), least, scale};
-  if (C > (1 << 30) || HW > (1 << 30) || B > (1 << 30)) return 1;
-  if (dtype == 0) return dropout_t<float>(key, x, y, Kc, B, C, HW, kind, inner, last, vec, st);
-  if (dtype == 1) return dropout_t<Bf16>(key, x, y, Kc, B, C, HW, kind, inner, last, vec, st);
-  return dropout_t<Half>(key, x, y, Kc, B, C, HW, kind, inner, last, vec, st);
+// What a layer's shape and key fix.  dtype 0 fp32, 1 bf16, 2 fp16.  kind 0 element, 1 channel, 2 sample.  last: channels-last
+// maps, else contiguous [.., C, HW].  inner: [B][Kc][C] instead of [Kc][B][C] in the leading dimensions.  least: smallest
+// 24-bit draw that is kept.
+struct DropPlan {
+  long B, C, HW;
+  unsigned long long seed;
+  int Kc, kind, inner, last, dtype;
+  unsigned c3, least;
+  float scale;
+};
+
+// tag null: tag_value.
+BLADES_API int blades_client_dropout(const void* x, void* y, const long* uids, const long* tag, long tag_value,
+                                     const DropPlan* p, hipStream_t st) {
+  if (p->Kc < 1 || p->B < 1 || p->C < 1 || p->HW < 1 || p->kind < 0 || p->kind > 2 || p->dtype < 0 || p->dtype > 2) return 1;
+  if ((double)p->B * p->C * p->HW > 1.7e10) return 1;  // draws of four are counted in 32 bits
+  if (p->C > (1 << 30) || p->HW > (1 << 30) || p->B > (1 << 30)) return 1;
+  const Key key{uids, tag, tag_value, p->c3, (uint32_t)p->seed, (uint32_t)(p->seed >> 32), p->least, p->scale};
+  const int vec = (((uintptr_t)x | (uintptr_t)y) & 15) == 0;  // 16-byte accesses (the lengths permitting)
+#define DROP(T) return dropout_t<T>(key, x, y, p->Kc, p->B, p->C, p->HW, p->kind, p->inner, p->last, vec, st)
+  if (p->dtype == 0) DROP(float);
+  if (p->dtype == 1) DROP(Bf16);
+  DROP(Half);
+#undef DROP
 }

@@ -44,6 +44,7 @@ struct Geo {
   int first, per_client;             // number of the launch's first sample in the batch, samples of a client
   int S, nslab, L, rows;             // channels of a slab, slabs, lanes of a pixel row, pixel rows at a time
   int chunk, nchunk;                 // pixels of a chunk, chunks of a sample
+  int through;                       // outputs past the caches (store_out)
   int back;                          // samples from the last one (the second sweep: what the first read last is still near)
   int pre, tw, tw_ch, tw_gr;         // see slab_sums
   int act;
@@ -180,7 +181,9 @@ __device__ __forceinline__ void normed(const Pack<T, VEC>& x, const float (&mu)[
 // ---------------------------------------------------------------------------------------------------------------
 inline int pow2_up(int v) { int p = 1; while (p < v) p <<= 1; return p; }
 
-struct Plan { Geo q; int threads, R, split, one; size_t lds; long piece; };
+struct Plan { Geo q; int threads, R, split, one; size_t lds; long piece, ws; };
+// both directions of a layer's shape
+struct Layer { Plan fwd, bwd; int dtype, vec; };
 
 // The launch of one direction (`hold`: vectors of registers per vector of the sample — 1 forward, 2 backward).
 // Returns false where no slab of whole groups fits a workgroup.
@@ -191,6 +194,11 @@ inline bool make_plan(Plan& pl, long N, long P, int C, int G, int esize, int vec
   q.per_client = per_client;
   q.first = 0;
   q.back = 0;
+  // Outputs of up to 256 MB, the last-level cache, are stored past it: 2048 x 128 x 16 x 16 bf16 (128 MB) forward 47 us
+  // against 51, backward 79 against 94 (with a producer and a consumer of equal size around them 134 against 142, 173
+  // against 183); 2048 x 512 x 4 x 4 fp32 (64 MB) 120 against 104 a pass alone, 61 against 64 forward in such a chain.
+  // Beyond it that costs: 2048 x 64 x 32 x 32 fp32 (512 MB) 538 us a pass against 554, in a chain 548 against 573 forward.
+  q.through = N * P * C * esize <= (256L << 20);
   // Slabs: as few as give workgroups of at most 256 threads x `maxr` vectors, but with pixel rows of at least a cache
   // line (128 bytes).  Narrower ones (down to 64 bytes) only where a sample would not fit a workgroup otherwise, and down
   // to single groups where the chip would stand half empty.  A sample that does not fit even so is split into chunks of

@@ -41,7 +41,7 @@ __device__ __forceinline__ void slope_vector(const Pack<T, VEC>& gy, const float
 template <typename T, int VEC, int NM>
 __device__ __forceinline__ void bwd_vector(const float (&g)[VEC], const float (&xh)[VEC], size_t o, T* dx, T* dres,
                                            const float (&rs)[NM], const float (&ga)[VEC], const float (&m1)[NM],
-                                           const float (&m2)[NM]) {
+                                           const float (&m2)[NM], bool through) {
   typedef Pack<T, VEC> V;
   if (dx != nullptr) {
     V w;
@@ -50,13 +50,13 @@ __device__ __forceinline__ void bwd_vector(const float (&g)[VEC], const float (&
       const int m = NM == 1 ? 0 : j;
       from_f(rs[m] * (fmaf(g[j], ga[j], -m1[m]) - xh[j] * m2[m]), w.e[j]);
     }
-    *reinterpret_cast<V*>(dx + o) = w;
+    store_out(dx + o, w, through);
   }
   if (dres != nullptr) {
     V w;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) from_f(g[j], w.e[j]);
-    *reinterpret_cast<V*>(dres + o) = w;
+    store_out(dres + o, w, through);
   }
 }
 
@@ -145,7 +145,7 @@ __global__ __launch_bounds__(MAX_THREADS) void gn_bwd_kernel(Geo q, const T* __r
       } else {
         slope_vector<T, VEC, AK>(gr[i], xh, o, res, gate, ga, be, q.act, g);
       }
-      bwd_vector<T, VEC, NM>(g, xh, o, dx, dres, rs, ga, m1, m2);
+      bwd_vector<T, VEC, NM>(g, xh, o, dx, dres, rs, ga, m1, m2, q.through);
     }
 }
 
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(MAX_THREADS) void gn_bwd_chunk_kernel(Geo q, const 
           normed<T, VEC, NM>(xr[i], mu, rs, xh);
           slope_vector<T, VEC, AK>(gr[i], xh, o + i * w.step, res, gate, ga, be, q.act, g);
           if (APPLY) {
-            bwd_vector<T, VEC, NM>(g, xh, o + i * w.step, dx, dres, rs, ga, m1, m2);
+            bwd_vector<T, VEC, NM>(g, xh, o + i * w.step, dx, dres, rs, ga, m1, m2, q.through);
           } else {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
@@ -327,29 +327,34 @@ int backward_t(const Plan& pl, const void* x, const void* res, const void* gy, c
 // dx / dres may be null.  dgamma / dbeta: rows of `ld` floats per client (an update matrix's rows or a [clients][C]
 // tensor), scaled by coef[client] (null: 1) and added to what is there where `accumulate`; null: not wanted.
 BLADES_API int blades_group_norm_backward(const void* x, const void* res, const void* gy, const void* gate, const float* gamma,
-                                          const float* beta, const float* mean, const float* rstd, long N, long P, int C,
-                                          int G, int act, int per_client, long gstride, long bstride, void* dx, void* dres,
-                                          const float* coef, float* dgamma, float* dbeta, long ld, int accumulate, float* ws,
-                                          int dtype, int vec, hipStream_t st) {
-  Plan pl;
-  if (!valid(N, P, C, G, vec, dtype, per_client) || act < 0 || act > 3) return 1;
-  if (!make_plan(pl, N, P, C, G, dtype == 0 ? 4 : 2, vec, 2, per_client)) return 2;
-  pl.q.eps = 0.f; pl.q.act = act; pl.q.gstride = gstride; pl.q.bstride = bstride;
+                                          const float* beta, const float* stats, void* dx, void* dres, const float* coef,
+                                          float* dgamma, float* dbeta, long ld, int accumulate, float* ws, const Layer* p,
+                                          hipStream_t st) {
+  const Plan& pl = p->bwd;
+  const Geo& q = pl.q;
+  const int act = q.act;
   const unsigned char* gt = (const unsigned char*)gate;
-  int rc;
-#define GN_B(T, V, M, K) rc = backward_t<T, V, M, K>(pl, x, res, gy, gt, gamma, beta, mean, rstd, dx, dres, ws, st)
+  const float *mean = stats, *rstd = stats + (size_t)q.N * (q.C / q.D);
+#define GN_B(T, V, M, K) backward_t<T, V, M, K>(pl, x, res, gy, gt, gamma, beta, mean, rstd, dx, dres, ws, st)
 #define GN_BT(T)                                                                                  \
-  if (vec == 1) GN_B(T, 1, 1, -1);                                                                \
+  if (p->vec == 1) GN_B(T, 1, 1, -1);                                                             \
   else if (act < 2) { if (pl.one) GN_B(T, 4, 1, 0); else GN_B(T, 4, 4, 0); }                      \
   else if (act == 2) { if (pl.one) GN_B(T, 4, 1, 2); else GN_B(T, 4, 4, 2); }                     \
   else { if (pl.one) GN_B(T, 4, 1, 3); else GN_B(T, 4, 4, 3); }
-  if (dtype == 0) { GN_BT(float) }
-  else if (dtype == 1) { GN_BT(Bf16) }
+  if (p->dtype == 0) { GN_BT(float) }
+  else if (p->dtype == 1) { GN_BT(Bf16) }
   else { GN_BT(Half) }
 #undef GN_BT
 #undef GN_B
-  if (rc == 0 && (dgamma != nullptr || dbeta != nullptr))
-    hipLaunchKernelGGL(gn_affine_kernel, dim3((unsigned)(N / per_client) * cdiv(C, AFF_CH)), dim3(AFF_CH * AFF_ROWS), 0, st,
-                       (const float2*)ws, per_client, C, coef, dgamma, dbeta, ld, accumulate);
-  return rc;
+  if (dgamma != nullptr || dbeta != nullptr) {
+    const int groups = cdiv(q.C, AFF_CH);
+    const long clients = q.N / q.per_client, most = ((1L << 32) - 1) / ((long)groups * AFF_CH * AFF_ROWS);
+    for (long k = 0; k < clients; k += most) {
+      const long n = clients - k < most ? clients - k : most;
+      hipLaunchKernelGGL(gn_affine_kernel, dim3((unsigned)(n * groups)), dim3(AFF_CH * AFF_ROWS), 0, st,
+                         (const float2*)ws + k * q.per_client * q.C, q.per_client, q.C, coef ? coef + k : nullptr,
+                         dgamma ? dgamma + k * ld : nullptr, dbeta ? dbeta + k * ld : nullptr, ld, accumulate);
+    }
+  }
+  return 0;
 }

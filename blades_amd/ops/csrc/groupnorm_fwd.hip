@@ -8,7 +8,7 @@ using namespace groupnorm;
 template <typename T, int VEC, int NM, int AK>
 __device__ __forceinline__ void fwd_vector(const Pack<T, VEC>& x, size_t o, const T* res, T* y, unsigned char* gate,
                                            const float (&mu)[NM], const float (&rs)[NM], const float (&ga)[VEC],
-                                           const float (&be)[VEC], int act) {
+                                           const float (&be)[VEC], int act, bool through) {
   typedef Pack<T, VEC> V;
   float z[VEC];
   normed<T, VEC, NM>(x, mu, rs, z);
@@ -28,7 +28,7 @@ __device__ __forceinline__ void fwd_vector(const Pack<T, VEC>& x, size_t o, cons
   V w;
 #pragma unroll
   for (int j = 0; j < VEC; ++j) from_f(act_f<AK>(z[j], act), w.e[j]);
-  *reinterpret_cast<V*>(y + o) = w;
+  store_out(y + o, w, through);
 }
 
 // Whole samples.  R vectors a thread.
@@ -87,7 +87,7 @@ __global__ __launch_bounds__(MAX_THREADS) void gn_fwd_kernel(Geo q, const T* __r
 #pragma unroll
   for (int i = 0; i < R; ++i)
     if (w.row + i * q.rows < w.pn)
-      fwd_vector<T, VEC, NM, AK>(xr[i], w.at + i * w.step, res, y, gate, mu, rs, ga, be, q.act);
+      fwd_vector<T, VEC, NM, AK>(xr[i], w.at + i * w.step, res, y, gate, mu, rs, ga, be, q.act, q.through);
 }
 
 // Pixel chunks, first sweep: (mean, M2) of a chunk.  A thread takes blocks of 4 vectors, centres each block's squares on
@@ -184,7 +184,7 @@ __global__ __launch_bounds__(MAX_THREADS) void gn_fwd_apply_kernel(Geo q, const 
 #pragma unroll
     for (int i = 0; i < BLOCK; ++i)
       if (p + i * q.rows < w.pn)
-        fwd_vector<T, VEC, NM, AK>(xr[i], o + i * w.step, res, y, gate, mu, rs, ga, be, q.act);
+        fwd_vector<T, VEC, NM, AK>(xr[i], o + i * w.step, res, y, gate, mu, rs, ga, be, q.act, q.through);
   }
 }
 
@@ -255,36 +255,44 @@ int forward_t(const Plan& pl, const void* x, const void* res, const float* gamma
 
 }  // namespace
 
-// dtype 0 fp32, 1 bf16, 2 fp16; vec: 4 channels per access, or 1 where C or an address does not allow it.
-// Workspace bytes of a direction (0 forward, 1 backward); -1: not supported (a group's channels exceed a workgroup).
-BLADES_API long blades_group_norm_ws(long N, long P, int C, int G, int dtype, int vec, int direction) {
-  Plan pl;
-  if (!valid(N, P, C, G, vec, dtype, 1)) return -1;
-  if (!make_plan(pl, N, P, C, G, dtype == 0 ? 4 : 2, vec, direction ? 2 : 1, 1)) return -1;
-  const long g = C / pl.q.D;
-  if (direction == 0) return pl.split ? pl.piece * pl.q.nchunk * g * 8 : 0;
-  return (N * C + (pl.split ? N * g + pl.piece * pl.q.nchunk * C : 0)) * 8;
+BLADES_API long blades_group_norm_plan_size() { return sizeof(Layer); }
+
+// What a layer's shape fixes.  dtype 0 fp32, 1 bf16, 2 fp16; vec: 4 channels per access, or 1 where C or an address does not
+// allow it.  gamma / beta: stride from client to client in floats (0: shared).  act 0 none, 1 ReLU, 2 GELU, 3 SiLU.
+// ws[2]: workspace bytes of the forward (0: a split sample's alone) and backward pass.
+// Returns 2 where the shape is not supported (a group's channels exceed a workgroup).
+BLADES_API int blades_group_norm_plan(Layer* p, long N, long P, int C, int G, float eps, int act, int per_client, long gstride,
+                                      long bstride, int dtype, int vec, long* ws) {
+  if (!valid(N, P, C, G, vec, dtype, per_client) || act < 0 || act > 3) return 1;
+  p->dtype = dtype; p->vec = vec;
+  for (int k = 0; k < 2; ++k) {
+    Plan& pl = k ? p->bwd : p->fwd;
+    if (!make_plan(pl, N, P, C, G, dtype == 0 ? 4 : 2, vec, k + 1, per_client)) return 2;
+    pl.q.eps = eps; pl.q.act = act; pl.q.gstride = gstride; pl.q.bstride = bstride;
+    pl.ws = k == 0 ? (pl.split ? pl.piece * pl.q.nchunk * G * 8 : 0)
+                   : (N * C + (pl.split ? N * G + pl.piece * pl.q.nchunk * C : 0)) * 8;
+    ws[k] = pl.ws;
+  }
+  return 0;
 }
 
-// gamma / beta: null, one vector (stride 0) or one per client (stride in floats).  mean / rstd [N][G]: may be null where
-// no backward pass follows (then not for a split plan: callers always pass them).  gate: one byte per vector, null: none.
-BLADES_API int blades_group_norm_forward(const void* x, const void* res, const float* gamma, const float* beta, long N, long P,
-                                         int C, int G, float eps, int act, int per_client, long gstride, long bstride, void* y,
-                                         void* gate, float* mean, float* rstd, float* ws, int dtype, int vec, hipStream_t st) {
-  Plan pl;
-  if (!valid(N, P, C, G, vec, dtype, per_client) || act < 0 || act > 3) return 1;
-  if (!make_plan(pl, N, P, C, G, dtype == 0 ? 4 : 2, vec, 1, per_client)) return 2;
-  pl.q.eps = eps; pl.q.act = act; pl.q.gstride = gstride; pl.q.bstride = bstride;
+// gamma / beta: null or one vector (per client).  stats [2][N][G]: mean, 1 / std; null where neither a backward pass nor a
+// workspace follows.  gate: one byte per vector, null: none.
+BLADES_API int blades_group_norm_forward(const void* x, const void* res, const float* gamma, const float* beta, void* y,
+                                         void* gate, float* stats, float* ws, const Layer* p, hipStream_t st) {
+  const Plan& pl = p->fwd;
+  const int act = pl.q.act;
   unsigned char* gt = (unsigned char*)gate;
+  float *mean = stats, *rstd = stats ? stats + (size_t)pl.q.N * (pl.q.C / pl.q.D) : nullptr;
 #define GN_F(T, V, M, K) return forward_t<T, V, M, K>(pl, x, res, gamma, beta, y, gt, mean, rstd, ws, st)
 #define GN_FT(T)                                                                                  \
-  if (vec == 1) GN_F(T, 1, 1, -1);                                                                \
+  if (p->vec == 1) GN_F(T, 1, 1, -1);                                                             \
   if (act < 2) { if (pl.one) GN_F(T, 4, 1, 0); GN_F(T, 4, 4, 0); }                                \
   if (act == 2) { if (pl.one) GN_F(T, 4, 1, 2); GN_F(T, 4, 4, 2); }                               \
   if (pl.one) GN_F(T, 4, 1, 3);                                                                   \
   GN_F(T, 4, 4, 3)
-  if (dtype == 0) { GN_FT(float); }
-  if (dtype == 1) { GN_FT(Bf16); }
+  if (p->dtype == 0) { GN_FT(float); }
+  if (p->dtype == 1) { GN_FT(Bf16); }
   GN_FT(Half);
 #undef GN_FT
 #undef GN_F

@@ -5,10 +5,12 @@
 // which is the gradient, a rotation's transpose).
 //
 // x [R][N][S][H][D] with any strides (D contiguous): slots s < rot of the packed projection are turned (q and k), the
-// others copied (v).  A thread owns 16 bytes of the head dimension of one token: its two (four) angles are computed once,
-// the turns (position times frequency in turns, reduced to an eighth) in 64 bits so that far positions keep theirs, sine
-// and cosine by their Taylor polynomials in 32 bits, and used for all slots and heads of the token.
-// Memory-bound: every byte is read and written once.
+// others copied (v).  A thread owns 16 bytes of the head dimension of one token: while its first rows are on their way, its two
+// (four) angles are computed, once for all its rows (slots and heads): the turns (position times frequency, reduced to an
+// eighth) in 64 bits so that far positions keep theirs, sine and cosine by their Taylor polynomials in 32 bits.
+// Memory-bound: every byte is read and written once.  (A workgroup that shares its tokens' angles through LDS and walks
+// memory in order was slower, 95 against 73 us on 2048 x 64 x 3 x 2 x 64 fp32: the index arithmetic of every vector and
+// half the waves cost more than the angles.)
 #include "common.h"
 
 namespace {
@@ -34,7 +36,7 @@ struct Shape {
   long R, N, sr, sn, ss, sh;       // samples, tokens; strides of x in elements (D: 1)
   int S, H, D, A, rot, slots;      // slots that are turned; slots that are walked (in place: the turned ones alone)
   long psr;                        // sample stride of the positions (0: shared)
-  int pos_float, inverse;
+  int pos_float, inverse, through;
 };
 
 // sine and cosine of a full turn's fraction
@@ -55,7 +57,7 @@ __device__ __forceinline__ void sincos_turns(double turns, float& s, float& c) {
 template <typename T, int VEC>
 __global__ __launch_bounds__(TPB) void rope_kernel(Freq f, Shape q, int per, const T* x, const void* __restrict__ pos, T* y) {
   typedef Pack<T, VEC> V;
-  constexpr int U = 4;
+  constexpr int U = 6;
   const int L = q.D / VEC;  // threads of a token
   const int r0 = blockIdx.y * per, r1 = min(r0 + per, q.slots * q.H);
   const bool turns = r0 < q.rot * q.H;
@@ -66,6 +68,19 @@ __global__ __launch_bounds__(TPB) void rope_kernel(Freq f, Shape q, int per, con
     const long r = token / q.N, n = token - r * q.N;
     const long xo = r * q.sr + n * q.sn + l * VEC;
     const size_t yo = (size_t)token * q.S * q.H * q.D + (size_t)l * VEC;
+    V w[U];
+    long at[U];
+    int s = r0 / q.H, h = r0 - s * q.H, turned[U];
+    auto fetch = [&](int row) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        at[u] = xo + s * q.ss + h * q.sh;
+        turned[u] = s < q.rot;
+        if (row + u < r1) w[u] = *reinterpret_cast<const V*>(x + at[u]);
+        if (++h == q.H) { h = 0; ++s; }
+      }
+    };
+    fetch(r0);
     float sn[VEC / 2], cs[VEC / 2];
     if (turns) {
 #pragma unroll
@@ -80,22 +95,11 @@ __global__ __launch_bounds__(TPB) void rope_kernel(Freq f, Shape q, int per, con
         }
       }
     }
-    int s = r0 / q.H, h = r0 - s * q.H;
-    for (int row = r0; row < r1; row += U) {
-      V w[U];
-      long at[U];
-      bool turn[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        at[u] = xo + s * q.ss + h * q.sh;
-        turn[u] = s < q.rot;
-        if (row + u < r1) w[u] = *reinterpret_cast<const V*>(x + at[u]);
-        if (++h == q.H) { h = 0; ++s; }
-      }
+    for (int row = r0;;) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (row + u < r1) {
-          if (turn[u]) {
+          if (turned[u]) {
 #pragma unroll
             for (int j = 0; j < VEC / 2; ++j) {
               const float a = to_f(w[u].e[2 * j]), b = to_f(w[u].e[2 * j + 1]);
@@ -103,43 +107,72 @@ __global__ __launch_bounds__(TPB) void rope_kernel(Freq f, Shape q, int per, con
               from_f(fmaf(a, sn[j], b * cs[j]), w[u].e[2 * j + 1]);
             }
           }
-          *reinterpret_cast<V*>(y + (same ? (size_t)at[u] : yo + (size_t)(row + u) * q.D)) = w[u];
+          store_out(y + (same ? (size_t)at[u] : yo + (size_t)(row + u) * q.D), w[u], q.through);
         }
+      row += U;
+      if (row >= r1) break;
+      fetch(row);
     }
   }
 }
+
+struct RopePlan {
+  Freq f;
+  Shape q;
+  int dtype, vec, blocks, per, per_in_place;
+};
+
+// A thread's rows: all of its token, fewer (at least 4) while the chip's 256 x 8 workgroups are not there.
+inline int rows_of(long blocks, int rows) {
+  int per = rows;
+  while (per > 4 && blocks * ((rows + per - 1) / per) < 2048) per = (per + 1) / 2;
+  return per;
+}
 }  // namespace
 
-// axes[A]: section widths (even, sum <= D).  y: contiguous [R][N][S][H][D], or x itself (then only the turned slots are
-// touched).  dtype 0 fp32, 1 bf16, 2 fp16; vec: elements per access (16 bytes, or 2 where an address does not allow it).
-BLADES_API int blades_rope_axes(const void* x, void* y, const void* pos, int pos_float, long psr, long R, long N, int S, int H,
-                                int D, long sr, long sn, long ss, long sh, int rot, const int* axes, int A, double base,
-                                int inverse, int dtype, int vec, hipStream_t st) {
+BLADES_API long blades_rope_plan_size() { return sizeof(RopePlan); }
+
+// What a layer's shape fixes.  axes[A]: section widths (even, sum <= D).  Strides of x in elements (D: 1).  dtype 0 fp32,
+// 1 bf16, 2 fp16; vec: elements per access (16 bytes, or 2 where an address or a stride does not allow it).
+BLADES_API int blades_rope_plan(RopePlan* p, int pos_float, long psr, long R, long N, int S, int H, int D, long sr, long sn,
+                                long ss, long sh, int rot, const int* axes, int A, double base, int dtype, int vec) {
   if (R < 1 || N < 1 || S < 1 || H < 1 || D < 2 || D > 2 * MAX_PAIRS || D % 2 || A < 1 || A > 8 || rot < 0 || rot > S) return 1;
   if (dtype < 0 || dtype > 2 || (vec != 2 && vec != (dtype == 0 ? 4 : 8)) || D % vec || !(base > 0.0)) return 1;
-  Freq f;
+  if ((double)S * H > 1e9) return 1;
   int pair = 0;
   for (int a = 0; a < A; ++a) {
     if (axes[a] < 2 || axes[a] % 2 || 2 * pair + axes[a] > D) return 1;
     for (int i = 0; i < axes[a] / 2; ++i, ++pair) {
-      f.turns[pair] = pow(base, -2.0 * i / axes[a]) * 0.15915494309189533577;
-      f.axis[pair] = (unsigned char)a;
+      p->f.turns[pair] = pow(base, -2.0 * i / axes[a]) * 0.15915494309189533577;
+      p->f.axis[pair] = (unsigned char)a;
     }
   }
-  for (; pair < MAX_PAIRS; ++pair) { f.turns[pair] = 0.0; f.axis[pair] = 255; }
-  const Shape q{R, N, sr, sn, ss, sh, S, H, D, A, rot, x == y ? rot : S, psr, pos_float, inverse};
-  long blocks = (R * N * (D / vec) + TPB - 1) / TPB;
-  if (blocks > (1L << 20)) blocks = 1L << 20;
-  // a thread's rows: all of its token, fewer (at least 4 at a time) while the chip's 256 x 8 workgroups are not there
-  const int rows = q.slots * H;
+  for (; pair < MAX_PAIRS; ++pair) { p->f.turns[pair] = 0.0; p->f.axis[pair] = 255; }
+  // Outputs of up to 256 MB, the last-level cache, are stored past it: 2048 x 64 x 3 x 2 x 64 fp32 62 us against 78 (with a
+  // producer and a consumer of equal size around it 201 against 212), 8 x 3136 x 3 x 6 x 64 bf16 23 against 27 (59, 61).
+  const long bytes = R * N * S * H * D * (dtype == 0 ? 4 : 2);
+  p->q = Shape{R, N, sr, sn, ss, sh, S, H, D, A, rot, S, psr, pos_float, 0, bytes <= (256L << 20)};
+  p->dtype = dtype; p->vec = vec;
+  const long blocks = (R * N * (D / vec) + TPB - 1) / TPB;
+  p->blocks = (int)(blocks > (1L << 20) ? 1L << 20 : blocks);
+  p->per = rows_of(p->blocks, S * H);
+  p->per_in_place = rows_of(p->blocks, rot * H);
+  return 0;
+}
+
+// y: contiguous [R][N][S][H][D], or x itself (then only the turned slots are touched).
+BLADES_API int blades_rope_axes(const void* x, void* y, const void* pos, const RopePlan* p, int inverse, hipStream_t st) {
+  Shape q = p->q;
+  q.inverse = inverse;
+  if (x == y) q.slots = q.rot;
+  const int rows = q.slots * q.H, per = x == y ? p->per_in_place : p->per;
   if (rows == 0) return 0;
-  int per = rows;
-  while (per > 4 && blocks * ((rows + per - 1) / per) < 2048) per = (per + 1) / 2;
-  const dim3 grid((unsigned)blocks, (unsigned)((rows + per - 1) / per)), block(TPB);
-#define ROPE(T, V) hipLaunchKernelGGL((rope_kernel<T, V>), grid, block, 0, st, f, q, per, (const T*)x, pos, (T*)y)
-  if (dtype == 0) { if (vec == 4) ROPE(float, 4); else ROPE(float, 2); }
-  else if (dtype == 1) { if (vec == 8) ROPE(Bf16, 8); else ROPE(Bf16, 2); }
-  else { if (vec == 8) ROPE(Half, 8); else ROPE(Half, 2); }
+  const dim3 grid((unsigned)p->blocks, (unsigned)((rows + per - 1) / per)), block(TPB);
+  if (grid.y > 65535) return 1;
+#define ROPE(T, V) hipLaunchKernelGGL((rope_kernel<T, V>), grid, block, 0, st, p->f, q, per, (const T*)x, pos, (T*)y)
+  if (p->dtype == 0) { if (p->vec == 4) ROPE(float, 4); else ROPE(float, 2); }
+  else if (p->dtype == 1) { if (p->vec == 8) ROPE(Bf16, 8); else ROPE(Bf16, 2); }
+  else { if (p->vec == 8) ROPE(Half, 8); else ROPE(Half, 2); }
 #undef ROPE
   return 0;
 }

@@ -15,29 +15,32 @@ first-order: a second backward pass raises.
 import torch
 from torch.autograd.function import once_differentiable
 
+import blades_amd.ops as _ops
+
 from . import reference as ref
 
 _ACTS = ("none", "relu", "gelu", "silu")
 _KINDS = ("elem", "channel", "sample")
 _POS = (torch.int64, torch.float32)
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _wrapped = torch._C._functorch.is_functorch_wrapped_tensor
-
-
-def _own_kernel(t: torch.Tensor) -> bool:
-    from blades_amd import ops
-
-    return t.is_cuda and not ops._FORCE_REFERENCE and not _wrapped(t)
+_grad_mode = torch.is_grad_enabled
+_kernels = None
 
 
 def _h():
-    from blades_amd import ops
+    global _kernels
+    if _kernels is None:
+        _kernels = _ops._h()
+    return _kernels
 
-    return ops._h()
 
-
-def _kernel_dtype(name, x):
-    if x.dtype not in _h()._DT_CODE:
-        raise ValueError(f"{name}: CUDA tensors must be fp32, bf16 or fp16, got {x.dtype}")
+def _own_kernel(name: str, t: torch.Tensor) -> bool:
+    if not t.is_cuda or _ops._FORCE_REFERENCE or _wrapped(t):
+        return False
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"{name}: CUDA tensors must be fp32, bf16 or fp16, got {t.dtype}")
+    return True
 
 
 def _first_order(backward):
@@ -45,8 +48,8 @@ def _first_order(backward):
     while a graph of the backward pass is being built."""
     guarded = once_differentiable(backward)
 
-    def call(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    def call(ctx, gy):
+        return guarded(ctx, gy) if _grad_mode() else backward(ctx, gy)
 
     return call
 
@@ -57,37 +60,39 @@ class _GroupNormFn(torch.autograd.Function):
         groups, eps, act = cfg
         w, b = _affine(weight), _affine(bias)
         clients = _clients(w, b)
-        y, stats, gate = _h().group_norm_forward(x, groups, w, b, eps, act, residual, clients, True, True)
+        y, stats, gate, plan = _h().group_norm_forward(x, groups, w, b, eps, act, residual, clients, True, True)
+        lead = None  # the types of affine vectors that are not fp32
+        if w is not None and weight.dtype != w.dtype or b is not None and bias.dtype != b.dtype:
+            lead = (None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+        ctx.cfg = (groups, act, clients, plan, lead)
         # the gate stands in for the residual; without one z is computed again, from x and a smooth activation's residual
-        ctx.cfg = (groups, act, clients, 0 if gate is None else gate[1])
-        ctx.save_for_backward(x, w, b, stats, residual if act in ("gelu", "silu") else None,
-                              None if gate is None else gate[0])
-        ctx.lead = (None if weight is None else weight.dtype, None if bias is None else bias.dtype)
+        ctx.save_for_backward(x, w, b, stats, residual if act in ("gelu", "silu") else None, gate)
         return y
 
     @staticmethod
     @_first_order
     def backward(ctx, gy):
         x, w, b, stats, res, gate = ctx.saved_tensors
-        groups, act, clients, gvec = ctx.cfg
+        groups, act, clients, plan, lead = ctx.cfg
         nx, nw, nb, nr, _ = ctx.needs_input_grad
-        dw = torch.empty(clients, x.shape[1], device=x.device) if nw else None
-        db = torch.empty(clients, x.shape[1], device=x.device) if nb else None
-        dx, dres = _h().group_norm_backward(x, gy, groups, w, b, stats, act, res, (gate, gvec) if gvec else None, clients, nx,
-                                            nr and act != "none", dw, db, x.shape[1], None, False, True)
+        dw = torch.empty(w.shape, device=x.device) if nw else None
+        db = torch.empty(b.shape, device=x.device) if nb else None
+        dx, dres = _kernels.group_norm_backward(x, gy, groups, w, b, stats, plan, act, res, gate, clients, nx,
+                                                nr and act != "none", dw, db, x.shape[1], None, False, True)
         if nr and act == "none":
             dres = gy
-        if nw:
-            dw = (dw if w.dim() == 2 else dw[0]).to(ctx.lead[0])
-        if nb:
-            db = (db if b.dim() == 2 else db[0]).to(ctx.lead[1])
+        if lead is not None:
+            dw = dw if dw is None else dw.to(lead[0])
+            db = db if db is None else db.to(lead[1])
         return dx, dw, db, dres, None
 
 
 def _affine(t):
     if t is None:
         return None
-    t = t.detach().to(torch.float32)
+    t = t.detach()
+    if t.dtype != torch.float32:
+        t = t.to(torch.float32)
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
@@ -99,7 +104,11 @@ def _clients(*affine):
 
 
 def _needs_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if _grad_mode():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def group_norm(x, groups: int, weight=None, bias=None, eps: float = 1e-5, act: str = "none", residual=None):
@@ -132,10 +141,7 @@ def group_norm(x, groups: int, weight=None, bias=None, eps: float = 1e-5, act: s
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
         raise ValueError(f"group_norm: residual must match x ({x.dtype} {tuple(x.shape)}), got {residual.dtype} "
                          f"{tuple(residual.shape)} on {residual.device}")
-    if not _own_kernel(x):
-        return ref.group_norm(x, groups, weight, bias, eps, act, residual)
-    _kernel_dtype("group_norm", x)
-    if x.numel() == 0:
+    if not _own_kernel("group_norm", x) or x.numel() == 0:
         return ref.group_norm(x, groups, weight, bias, eps, act, residual)
     if _needs_grad(x, weight, bias, residual):
         return _GroupNormFn.apply(x, weight, bias, residual, (groups, eps, act))
@@ -146,21 +152,28 @@ def group_norm(x, groups: int, weight=None, bias=None, eps: float = 1e-5, act: s
 class _ClientDropoutFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, uids, tag, cfg):
-        ctx.cfg, ctx.tag = cfg, tag
+        h = _h()
+        x, plan = h.dropout_plan(x, uids, *cfg)
         # the ids and the tag are saved, so that changing them between the two passes raises instead of drawing another mask
-        if torch.is_tensor(tag):
-            ctx.save_for_backward(uids, tag)
-            ctx.tag = None
-        else:
+        if type(tag) is int:
             ctx.save_for_backward(uids)
-        return _h().client_dropout(x, uids, cfg[0], tag, *cfg[1:], True)
+            ctx.run = (plan, x.stride(), cfg, tag)
+        else:
+            ctx.save_for_backward(uids, tag)
+            ctx.run = (plan, x.stride(), cfg, None)
+        return h.dropout_launch(x, uids, tag, plan)
 
     @staticmethod
     @_first_order
     def backward(ctx, gy):
-        uids, *tag = ctx.saved_tensors
-        cfg = ctx.cfg
-        return _h().client_dropout(gy, uids, cfg[0], tag[0] if tag else ctx.tag, *cfg[1:], True), None, None, None
+        plan, stride, cfg, tag = ctx.run
+        if tag is None:
+            uids, tag = ctx.saved_tensors
+        else:
+            (uids,) = ctx.saved_tensors
+        if gy.stride() != stride:
+            gy, plan = _h().dropout_plan(gy, uids, *cfg)
+        return _kernels.dropout_launch(gy, uids, tag, plan), None, None, None
 
 
 def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "elem", layout: str = "major", scale=None):
@@ -191,17 +204,17 @@ def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "e
         raise ValueError(f"client_dropout: {tuple(x.shape)} does not divide among {K} clients (layout {layout})")
     if x.numel() == 0:
         return x.clone()
-    if not _own_kernel(x):
+    if not _own_kernel("client_dropout", x):
         return ref.client_dropout(x, uids, seed, tag, layer, p, kind, layout, scale)
-    _kernel_dtype("client_dropout", x)
-    cfg = (int(seed), int(layer), p, kind, layout, None if scale is None else float(scale))
+    cfg = (int(seed), int(layer), p, kind, layout, None if scale is None else float(scale))  # (dropout_plan's)
     if uids.dim() == 0 or not uids.is_contiguous():
         uids = uids.reshape(-1).contiguous()
     if by_value:
         tag = int(tag)
-    if x.requires_grad and torch.is_grad_enabled():
+    if x.requires_grad and _grad_mode():
         return _ClientDropoutFn.apply(x, uids, tag, cfg)
-    return _h().client_dropout(x, uids, cfg[0], tag, *cfg[1:], True)
+    x, plan = _h().dropout_plan(x, uids, *cfg)
+    return _kernels.dropout_launch(x, uids, tag, plan)
 
 
 class _RopeFn(torch.autograd.Function):
@@ -243,9 +256,8 @@ def rope_axes(x, pos, axes, base: float = 10000.0, slots=None):
             len(shape) == 3 and shape[0] != x.shape[0]) or pos.device != x.device or pos.requires_grad:
         raise ValueError(f"rope_axes: pos must be int64 or fp32 [{x.shape[1]}, {len(axes)}] or [{x.shape[0]}, {x.shape[1]}, "
                          f"{len(axes)}] on {x.device} without a gradient, got {pos.dtype} {tuple(shape)} on {pos.device}")
-    if not _own_kernel(x):
+    if not _own_kernel("rope_axes", x):
         return ref.rope_axes(x, pos, axes, base, slots)
-    _kernel_dtype("rope_axes", x)
-    if x.requires_grad and torch.is_grad_enabled():
+    if x.requires_grad and _grad_mode():
         return _RopeFn.apply(x, pos, (axes, base, slots))
     return _h().rope_axes(x, pos, axes, base, slots, False, None, True)
