@@ -2010,8 +2010,8 @@ def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "e
         if torch.is_tensor(tag) and not (tag.device == x.device and tag.dtype == torch.int64 and tag.numel() == 1):
             raise ValueError("client_dropout: tag must be an int or a 1-element int64 tensor on x's device")
         tag = tag if torch.is_tensor(tag) else int(tag)
-        if not 0.0 <= p < 1.0:
-            raise ValueError("client_dropout: need 0 <= p < 1")
+        if not 0.0 <= c_float(p).value < 1.0:
+            raise ValueError("client_dropout: need 0 <= p < 1 in 32 bits")
     if x.numel() == 0:
         return x.clone()
     x, plan = dropout_plan(x, uids, seed, layer, p, kind, layout, scale)

@@ -48,6 +48,18 @@ template <typename V> __device__ __forceinline__ void store_out(void* p, const V
   *(V*)p = v;
 }
 
+// n / d for n < 2^31 by a multiplication (Granlund and Montgomery, "Division by invariant integers")
+struct Div {
+  uint32_t d, m, s;
+  static Div of(uint32_t d) {
+    Div r{d, 0, 0};
+    while ((1ull << r.s) < d) ++r.s;
+    r.m = (uint32_t)(((1ull << 32) * ((1ull << r.s) - d)) / d + 1);
+    return r;
+  }
+  __device__ __forceinline__ uint32_t over(uint32_t n) const { return (__umulhi(n, m) + n) >> s; }
+};
+
 static inline int cdiv(long a, long b) { return (int)((a + b - 1) / b); }
 
 // Philox4x32-10 — bit-identical to ops/reference.py::_philox4x32.

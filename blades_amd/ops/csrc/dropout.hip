@@ -26,15 +26,14 @@ struct Key {
   const long* uids;
   const long* tag;  // null: tag_value
   long tag_value;
-  uint32_t c3, k0, k1, least;  // least: smallest 24-bit draw that is kept
+  uint32_t c3, k0, k1, least;  // least: smallest word that is kept (the smallest kept 24-bit draw, 8 zero bits below)
   float scale;
 };
 
 // keep bits of the values 4q .. 4q + 3
 __device__ __forceinline__ unsigned keep4(const Key& key, uint32_t q, uint32_t uid, uint32_t tag) {
   const Philox4 r = philox4x32_10(q, uid, tag, key.c3, key.k0, key.k1);
-  return ((r.x >> 8) >= key.least ? 1u : 0u) | ((r.y >> 8) >= key.least ? 2u : 0u) | ((r.z >> 8) >= key.least ? 4u : 0u) |
-         ((r.w >> 8) >= key.least ? 8u : 0u);
+  return (r.x >= key.least ? 1u : 0u) | (r.y >= key.least ? 2u : 0u) | (r.z >= key.least ? 4u : 0u) | (r.w >= key.least ? 8u : 0u);
 }
 __device__ __forceinline__ uint32_t tag_of(const Key& key) { return (uint32_t)(key.tag ? key.tag[0] : key.tag_value); }
 
@@ -93,11 +92,83 @@ __global__ __launch_bounds__(TPB) void drop_elem_kernel(Key key, const T* __rest
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// A draw for every channel of a sample (kind 1) or every sample (2): every vector's thread makes its own, which costs less
-// than waiting for another's.  Memory is [..][dims], walked by vectors of VEC channels (LAST: [sample][pixel][client if
+// A draw for every channel of a sample (kind 1) or every sample (2), shared by its pixels.  Memory is outer rows of Ct
+// channels: samples of C channels, or (inner) a batch index's Kc * C; LAST: pixels first, [pixel][Ct], else [Ct][pixel].  A
+// workgroup takes `ns` whole rows, or (ns = 1) `cv` vectors of a large one: its first U vectors a thread are on their way while
+// the rows' draws go to LDS, a byte per channel.  (A draw by every vector's thread instead: 12.8 us against 9.7 for 3840 x 64
+// x 6 x 6 bf16, the generator bound.)
+constexpr int GROUP_BYTES = 16384;
+struct Rows {
+  long outer;                // rows
+  int Kc, B, C, Ct, HW, inner, kind;
+  int ns, cv, chunks, quads; // quads: C is a multiple of 4, draws come in fours
+  long nv;                   // vectors of a row
+  Div by_ct, by_hw, by_nv;   // by_hw: pixels in vectors
+};
+template <typename T, int VEC, bool LAST>
+__global__ __launch_bounds__(TPB) void drop_group_kernel(Key key, Rows q, const T* __restrict__ x, T* __restrict__ y) {
+  typedef Pack<T, VEC> V;
+  constexpr int U = 4;
+  __shared__ alignas(16) unsigned char keep[GROUP_BYTES];
+  const uint32_t tag = tag_of(key);
+  const long tiles = (q.outer + q.ns - 1) / q.ns * q.chunks;
+  for (long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const long t = tile / q.chunks, o0 = t * q.ns;
+    const int rows = (int)(q.outer - o0 < q.ns ? q.outer - o0 : q.ns);
+    const long v0 = (tile - t * q.chunks) * q.cv;
+    const int items = (int)(q.ns > 1 || q.chunks == 1 ? rows * q.nv : (q.nv - v0 < q.cv ? q.nv - v0 : q.cv));
+    const V* src = reinterpret_cast<const V*>(x) + o0 * q.nv + v0;
+    V* dst = reinterpret_cast<V*>(y) + o0 * q.nv + v0;
+    V w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if ((int)threadIdx.x + u * TPB < items) w[u] = src[threadIdx.x + u * TPB];
+    // channels of a row that these vectors touch
+    const int lo = LAST ? 0 : (int)(v0 / q.by_hw.d) & ~3;
+    const int hi = LAST || q.chunks == 1 ? q.Ct : min(q.Ct, (int)((v0 + items - 1) / q.by_hw.d) + 1);
+    const int step = q.quads ? 4 : 1, per = (hi - lo + step - 1) / step;
+    for (int i = threadIdx.x; i < rows * per; i += TPB) {
+      const int r = i / per, ch = lo + (i - r * per) * step;
+      const long o = o0 + r;
+      const int k = (int)(q.inner ? ch / q.C : o / q.B), c = q.inner ? ch - k * q.C : ch;
+      const long b = q.inner ? o : o - (long)k * q.B, e = q.kind == 2 ? b : b * q.C + c;
+      unsigned m = keep4(key, (uint32_t)(e >> 2), (uint32_t)key.uids[k], tag);
+      unsigned char* at = keep + r * q.Ct + ch;
+      if (q.quads) {
+        if (q.kind == 2) m = (m >> (e & 3)) & 1u ? 15u : 0u;
+        *reinterpret_cast<unsigned*>(at) = (m & 1u) | (m & 2u) << 7 | (m & 4u) << 14 | (m & 8u) << 21;
+      } else {
+        *at = (unsigned char)((m >> (e & 3)) & 1u);
+      }
+    }
+    __syncthreads();
+    auto finish = [&](V v, uint32_t i) {
+      const uint32_t r = q.ns > 1 ? q.by_nv.over(i) : 0u, f = i - r * (uint32_t)q.nv;  // (ns > 1: rows begin at v0 = 0)
+      const unsigned char* row = keep + r * q.Ct;
+      if (LAST) {
+        const uint32_t g = (uint32_t)((v0 * VEC) % q.Ct) + f * VEC, ch = g - q.by_ct.over(g) * q.Ct;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) from_f(to_f(v.e[j]) * (row[ch + j] ? key.scale : 0.f), v.e[j]);
+      } else {
+        const uint32_t first = (uint32_t)(v0 % q.by_hw.d), ch = (uint32_t)(v0 / q.by_hw.d) + q.by_hw.over(first + f);
+        const float s = row[ch] ? key.scale : 0.f;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) from_f(to_f(v.e[j]) * s, v.e[j]);
+      }
+      dst[i] = v;
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if ((int)threadIdx.x + u * TPB < items) finish(w[u], threadIdx.x + u * TPB);
+    for (int i = threadIdx.x + U * TPB; i < items; i += TPB) finish(src[i], i);
+    __syncthreads();  // the next tile's draws overwrite these
+  }
+}
+
+// The same for rows of more channels than a workgroup keeps: every vector's thread makes its own draws.  Memory is walked by vectors of VEC channels (LAST: [sample][pixel][client if
 // inner][C]) or of one channel's pixels (else: [sample][C][pixel]); index arithmetic in I bits.
 template <typename T, int VEC, bool LAST, typename I>
-__global__ __launch_bounds__(TPB) void drop_group_kernel(Key key, const T* __restrict__ x, T* __restrict__ y, int Kc, I B, I C,
+__global__ __launch_bounds__(TPB) void drop_wide_kernel(Key key, const T* __restrict__ x, T* __restrict__ y, int Kc, I B, I C,
                                                          I HW, int inner, int kind, I total) {
   typedef Pack<T, VEC> V;
   constexpr int U = 2;
@@ -214,17 +285,41 @@ int elem_t(const Key& key, const void* x, void* y, long nblk, int Kc, int inner,
 }
 
 template <typename T, int VEC, bool LAST>
-int group_v(const Key& key, const void* x, void* y, int Kc, long B, long C, long HW, int inner, int kind, hipStream_t st) {
+int wide_v(const Key& key, const void* x, void* y, int Kc, long B, long C, long HW, int inner, int kind, hipStream_t st) {
   const long elems = Kc * B * C * HW, total = elems / VEC;
   long gx = (total + 2 * TPB - 1) / (2 * TPB);
   if (gx > 8192) gx = 8192;
   const dim3 grid((unsigned)gx), block(TPB);
   if (elems < (1L << 31))  // (a stride of the grid beyond the end still fits 32 bits)
-    hipLaunchKernelGGL((drop_group_kernel<T, VEC, LAST, uint32_t>), grid, block, 0, st, key, (const T*)x, (T*)y, Kc, (uint32_t)B,
+    hipLaunchKernelGGL((drop_wide_kernel<T, VEC, LAST, uint32_t>), grid, block, 0, st, key, (const T*)x, (T*)y, Kc, (uint32_t)B,
                        (uint32_t)C, (uint32_t)HW, inner, kind, (uint32_t)total);
   else
-    hipLaunchKernelGGL((drop_group_kernel<T, VEC, LAST, long>), grid, block, 0, st, key, (const T*)x, (T*)y, Kc, B, C, HW, inner,
+    hipLaunchKernelGGL((drop_wide_kernel<T, VEC, LAST, long>), grid, block, 0, st, key, (const T*)x, (T*)y, Kc, B, C, HW, inner,
                        kind, total);
+  return 0;
+}
+
+template <typename T, int VEC, bool LAST>
+int group_v(const Key& key, const void* x, void* y, int Kc, long B, long C, long HW, int inner, int kind, hipStream_t st) {
+  Rows q;
+  q.Kc = Kc; q.B = (int)B; q.C = (int)C; q.HW = (int)HW; q.inner = inner; q.kind = kind;
+  const long Ct = inner ? Kc * C : C;
+  if (Ct > GROUP_BYTES || Ct * HW >= (1L << 31)) return wide_v<T, VEC, LAST>(key, x, y, Kc, B, C, HW, inner, kind, st);
+  q.outer = inner ? B : Kc * B;
+  q.Ct = (int)Ct;
+  q.nv = Ct * HW / VEC;
+  q.quads = C % 4 == 0;
+  constexpr int want = TPB * 8;
+  long ns = want / q.nv, most = GROUP_BYTES / Ct;
+  if (ns > most) ns = most;
+  if (ns > q.outer / 1024) ns = q.outer / 1024;  // (1024 workgroups first)
+  q.ns = (int)(ns < 1 ? 1 : ns);
+  q.cv = want;
+  q.chunks = q.ns > 1 || q.nv <= want ? 1 : (int)((q.nv + want - 1) / want);
+  q.by_ct = Div::of((uint32_t)Ct); q.by_hw = Div::of((uint32_t)(LAST ? HW : HW / VEC)); q.by_nv = Div::of((uint32_t)q.nv);
+  long tiles = (q.outer + q.ns - 1) / q.ns * q.chunks;
+  if (tiles > (1L << 20)) tiles = 1L << 20;
+  hipLaunchKernelGGL((drop_group_kernel<T, VEC, LAST>), dim3((unsigned)tiles), dim3(TPB), 0, st, key, q, (const T*)x, (T*)y);
   return 0;
 }
 
@@ -258,11 +353,11 @@ int dropout_t(const Key& key, const void* x, void* y, int Kc, long B, long C, lo
     const long nblk = inner ? Kc * B : Kc, len = inner ? C * HW : B * C * HW;
     return elem_t<T>(key, x, y, nblk, Kc, inner, len, vec && len % W == 0, st);
   }
+  if (kind == 2 && !inner) { HW *= C; C = 1; last = 0; }  // a sample is one run of memory: one channel
   if (last) {
     if (vec && C % W == 0) return group_v<T, W, true>(key, x, y, Kc, B, C, HW, inner, kind, st);
     return group_v<T, 1, true>(key, x, y, Kc, B, C, HW, inner, kind, st);
   }
-  if (kind == 2) { HW *= C; C = 1; }  // (a sample is one run of memory)
   if (vec && HW % W == 0) return group_v<T, W, false>(key, x, y, Kc, B, C, HW, inner, kind, st);
   return group_v<T, 1, false>(key, x, y, Kc, B, C, HW, inner, kind, st);
 }
@@ -270,7 +365,7 @@ int dropout_t(const Key& key, const void* x, void* y, int Kc, long B, long C, lo
 
 // What a layer's shape and key fix.  dtype 0 fp32, 1 bf16, 2 fp16.  kind 0 element, 1 channel, 2 sample.  last: channels-last
 // maps, else contiguous [.., C, HW].  inner: [B][Kc][C] instead of [Kc][B][C] in the leading dimensions.  least: smallest
-// 24-bit draw that is kept.
+// 24-bit draw that is kept, below 2^24.
 struct DropPlan {
   long B, C, HW;
   unsigned long long seed;
@@ -282,10 +377,10 @@ struct DropPlan {
 // tag null: tag_value.
 BLADES_API int blades_client_dropout(const void* x, void* y, const long* uids, const long* tag, long tag_value,
                                      const DropPlan* p, hipStream_t st) {
-  if (p->Kc < 1 || p->B < 1 || p->C < 1 || p->HW < 1 || p->kind < 0 || p->kind > 2 || p->dtype < 0 || p->dtype > 2) return 1;
+  if (p->Kc < 1 || p->B < 1 || p->C < 1 || p->HW < 1 || p->kind < 0 || p->kind > 2 || p->dtype < 0 || p->dtype > 2 || p->least >> 24) return 1;
   if ((double)p->B * p->C * p->HW > 1.7e10) return 1;  // draws of four are counted in 32 bits
   if (p->C > (1 << 30) || p->HW > (1 << 30) || p->B > (1 << 30)) return 1;
-  const Key key{uids, tag, tag_value, p->c3, (uint32_t)p->seed, (uint32_t)(p->seed >> 32), p->least, p->scale};
+  const Key key{uids, tag, tag_value, p->c3, (uint32_t)p->seed, (uint32_t)(p->seed >> 32), p->least << 8, p->scale};
   const int vec = (((uintptr_t)x | (uintptr_t)y) & 15) == 0;  // 16-byte accesses (the lengths permitting)
 #define DROP(T) return dropout_t<T>(key, x, y, p->Kc, p->B, p->C, p->HW, p->kind, p->inner, p->last, vec, st)
   if (p->dtype == 0) DROP(float);

@@ -21,6 +21,7 @@ from . import reference as ref
 
 _ACTS = ("none", "relu", "gelu", "silu")
 _KINDS = ("elem", "channel", "sample")
+_P_END = 1.0 - 2.0 ** -25  # rounds to 1 in 32 bits from here
 _POS = (torch.int64, torch.float32)
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _wrapped = torch._C._functorch.is_functorch_wrapped_tensor
@@ -190,8 +191,8 @@ def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "e
     if kind not in _KINDS or layout not in ("major", "inner"):
         raise ValueError(f"client_dropout: kind must be one of {_KINDS}, layout major or inner, got {kind!r}, {layout!r}")
     p = float(p)
-    if not 0.0 <= p < 1.0:
-        raise ValueError(f"client_dropout: need 0 <= p < 1, got {p}")
+    if not 0.0 <= p < _P_END:
+        raise ValueError(f"client_dropout: need 0 <= p < 1 in 32 bits, got {p}")
     K, by_value = uids.numel(), not torch.is_tensor(tag)
     if uids.dtype != torch.int64 or uids.dim() > 1 or K < 1 or uids.device != x.device:
         raise ValueError("client_dropout: uids must be an int64 vector (or scalar) of clients on x's device")

@@ -307,6 +307,7 @@ def drop_mask(uids, shape, seed, tag, layer, p, kind, layout):
 DROP_CASES = [  # shape per client and sample, clients, batch
     ((128,), 6, 8), ((7,), 3, 5), ((1,), 1, 1), ((13, 9), 4, 3), ((64, 32), 2, 4), ((5, 7, 3), 3, 2), ((64, 6, 6), 2, 5),
     ((3, 32, 32), 2, 2), ((65, 9, 30), 2, 2), ((130, 1, 1), 2, 3), ((8, 2, 2), 33, 1), ((2, 300, 40), 1, 2),
+    ((64, 6, 6), 30, 40), ((6, 50, 70), 2, 3), ((512, 2, 2), 40, 1), ((16, 8), 5, 300),
 ]
 
 
@@ -381,7 +382,7 @@ def test_client_dropout_changed_tag_raises(dev):
     (torch.zeros(4, 2, dtype=torch.int64), torch.arange(2), {}), (torch.zeros(5, 2), torch.arange(2), {}),
     (torch.zeros(4, 3), torch.arange(2), {"layout": "inner"}), (torch.zeros(4), torch.arange(2), {"layout": "inner"}),
     (torch.zeros(4, 2), torch.arange(2), {"kind": "row"}), (torch.zeros(4, 2), torch.arange(2), {"layout": "outer"}),
-    (torch.zeros(4, 2), torch.arange(2), {"p": 1.0}), (torch.zeros(4, 2), torch.arange(2), {"p": -0.1}),
+    (torch.zeros(4, 2), torch.arange(2), {"p": 1.0}), (torch.zeros(4, 2), torch.arange(2), {"p": 1 - 2.0 ** -25}), (torch.zeros(4, 2), torch.arange(2), {"p": -0.1}),
     (torch.zeros(4, 2), torch.arange(2), {"p": float("nan")}), (torch.zeros(4, 2), torch.zeros(2), {}),
     (torch.zeros(4, 2), torch.zeros(0, dtype=torch.int64), {}), (torch.zeros(4, 2), torch.zeros(2, 1, dtype=torch.int64), {}),
     (torch.zeros(4, 2), torch.arange(2), {"tag": torch.zeros(2, dtype=torch.int64)}),
