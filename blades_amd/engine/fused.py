@@ -741,19 +741,26 @@ class _MHAFn(torch.autograd.Function):
     (sample, head) in one kernel; backward recomputes the probabilities from the saved row log-sum-exp."""
 
     @staticmethod
-    def forward(ctx, qkv, B, scale, drop, npl):
+    def forward(ctx, qkv, B, scale, drop, npl, rope=None):
         h = _hipmod()
         uids, tag, seed, layer, p = drop if drop is not None else (None, None, 0, 0, 0.0)
+        if rope is not None:  # queries and keys turned by their positions (ops/csrc/rope.hip)
+            qkv = h.rope_axes(qkv, rope.pos, rope.axes, rope.base, 2)
         o, lse = h.mha_forward(qkv, B, scale, uids, tag, seed, layer, p, npl)
         ctx.save_for_backward(qkv, o, lse)
         ctx.cfg = (B, scale, uids, tag, seed, layer, p, npl)
+        ctx.rope = rope
         return o
 
     @staticmethod
     def backward(ctx, d_o):
         qkv, o, lse = ctx.saved_tensors
         B, scale, uids, tag, seed, layer, p, npl = ctx.cfg
-        return _hipmod().mha_backward(qkv, o, d_o, lse, B, scale, uids, tag, seed, layer, p, npl), None, None, None, None
+        dqkv = _hipmod().mha_backward(qkv, o, d_o, lse, B, scale, uids, tag, seed, layer, p, npl)
+        if ctx.rope is not None:  # turned back where it lies: nobody else holds this tensor, and v's third stays untouched
+            r = ctx.rope
+            _hipmod().rope_axes(dqkv, r.pos, r.axes, r.base, 2, inverse=True, out=dqkv)
+        return dqkv, None, None, None, None, None
 
 
 class PCAttention(nn.Module):
@@ -768,6 +775,7 @@ class PCAttention(nn.Module):
         self.attn_drop = attn.attn_drop
         self.proj = attn.proj
         self.proj_drop = attn.proj_drop
+        self.rope = attn.rope
 
     def _drop_cfg(self):
         d = self.attn_drop
@@ -791,8 +799,9 @@ class PCAttention(nn.Module):
         q5 = qkv.reshape(Bn, N, 3, H, C // H)
         if ok and x.is_cuda and _os.environ.get("BLADES_DISABLE_HIP_MHA") != "1" and _hipmod().mha_supported(q5) \
                 and Bn % max(self.sink.Kc, 1) == 0:
-            o = _MHAFn.apply(q5, Bn // max(self.sink.Kc, 1), float(self.scale), drop, self.sink.npl)
+            o = _MHAFn.apply(q5, Bn // max(self.sink.Kc, 1), float(self.scale), drop, self.sink.npl, self.rope)
         else:
+            q5 = q5 if self.rope is None else self.rope(q5)
             q, k, v = q5.permute(2, 0, 3, 1, 4)
             attn = self.attn_drop(((q @ k.transpose(-2, -1)) * self.scale).softmax(dim=-1))
             o = (attn @ v).transpose(1, 2).reshape(Bn, N, C)
@@ -938,6 +947,85 @@ class PCBatchNorm2d(nn.Module):
         return y
 
 
+class _PCGroupNormFn(torch.autograd.Function):
+    """Group norm with fused residual add and activation (ops/csrc/groupnorm.hip); each client's affine gradients go,
+    scaled, into its update row.  Statistics are a sample's own, so clients matter to the affine pair alone.  Shapes the
+    kernel does not take, and the CPU, run the oracle, the backward pass through autograd on it."""
+
+    @staticmethod
+    def forward(ctx, x, res, anchor, mod, act):
+        sink: GradSink = mod.sink
+        w, b = sink.param(mod.weight), sink.param(mod.bias)
+        ctx.mod, ctx.act, ctx.has_res = mod, act, res is not None
+        Kc = sink.Kc if mod.weight is not None else 1
+        ctx.hip = x.is_cuda and _hipmod().group_norm_supported(x, mod.num_groups)
+        if ctx.hip:
+            w, b = (t if t is None else t.detach().float() for t in (w, b))
+            y, stats, gate, plan = _hipmod().group_norm_forward(x, mod.num_groups, w, b, mod.eps, act, res, Kc,
+                                                                for_backward=any(ctx.needs_input_grad))
+            ctx.plan, ctx.affine = plan, (w, b)
+            ctx.save_for_backward(x, res if act in ("gelu", "silu") else None, stats, gate)
+            return y
+        from blades_amd.ops import reference as ref
+
+        ctx.save_for_backward(x, res)
+        return ref.group_norm(x, mod.num_groups, w, b, mod.eps, act, res)
+
+    @staticmethod
+    def backward(ctx, gy):
+        mod, act = ctx.mod, ctx.act
+        sink: GradSink = mod.sink
+        Kc = sink.Kc if mod.weight is not None else 1
+        want_dx, want_dres = ctx.needs_input_grad[0], ctx.has_res and ctx.needs_input_grad[1]
+        if ctx.hip:
+            x, res, stats, gate = ctx.saved_tensors
+            w, b = ctx.affine
+            dw = db = None
+            acc, ld = False, 0
+            if mod.weight is not None:
+                acc = id(mod.weight) in sink._written
+                sink._written.add(id(mod.weight))
+                sink._written.add(id(mod.bias))
+                dw, db = sink.view(mod.weight), sink.view(mod.bias)
+                ld = max(int(sink.block.stride(0)), int(dw.shape[1]))
+            dx, dres = _hipmod().group_norm_backward(x, gy.to(x.dtype), mod.num_groups, w, b, stats, ctx.plan, act, res, gate,
+                                                     Kc, want_dx, want_dres and act != "none", dw, db, ld,
+                                                     None if dw is None else sink.scale, acc)
+            return dx, (gy if act == "none" else dres) if want_dres else None, None, None, None
+        from blades_amd.ops import reference as ref
+
+        x, res = ctx.saved_tensors
+        C = x.shape[1]
+        with torch.enable_grad():
+            xs = x.detach().requires_grad_(True)
+            rs = None if res is None else res.detach().requires_grad_(True)
+            w = b = None
+            if mod.weight is not None:  # one pair per client, so that the gradients come per client
+                w, b = (sink.param(t).detach().float().expand(Kc, C).clone().requires_grad_(True)
+                        for t in (mod.weight, mod.bias))
+            y = ref.group_norm(xs, mod.num_groups, w, b, mod.eps, act, rs)
+        leaves = [t for t in (xs, rs, w, b) if t is not None]
+        got = dict(zip(map(id, leaves), torch.autograd.grad(y, leaves, gy)))
+        if mod.weight is not None:
+            sink.write(mod.weight, got[id(w)])
+            sink.write(mod.bias, got[id(b)])
+        return got[id(xs)] if want_dx else None, got[id(rs)] if want_dres else None, None, None, None
+
+
+class PCGroupNorm(nn.Module):
+    def __init__(self, gn: nn.GroupNorm, sink: GradSink, act: str = "none"):
+        super().__init__()
+        self.num_groups, self.eps, self.sink, self.act = gn.num_groups, gn.eps, sink, act
+        self.weight, self.bias = gn.weight, gn.bias
+
+    def extra_repr(self):
+        return f"{self.num_groups}, activation_folded={self.act}"
+
+    def forward(self, x, residual=None, relu: bool = False):
+        anchor = self.weight if self.weight is not None else x
+        return _PCGroupNormFn.apply(x, residual, anchor, self, "relu" if relu else self.act)
+
+
 def _conv_bn(conv, bn, x, residual=None, relu: bool = False, join=None, sole: bool = False):
     """``bn(conv(x))`` with the BatchNorm statistics taken from the convolution kernel's epilogue when both are
     the engine's own modules (no separate statistics pass over the convolution output)."""
@@ -945,7 +1033,8 @@ def _conv_bn(conv, bn, x, residual=None, relu: bool = False, join=None, sole: bo
         y = conv(x, want_stats=True, join=join, sole=sole)
         pre, conv.bn_stats = conv.bn_stats, None
         return bn(y, residual=residual, relu=relu, pre_stats=pre)
-    return bn(conv(x), residual=residual, relu=relu)
+    y = conv(x, join=join, sole=sole) if isinstance(conv, PCConv2d) else conv(x)
+    return bn(y, residual=residual, relu=relu)
 
 
 class PCResBlock(nn.Module):
@@ -1010,7 +1099,7 @@ def supports(model: nn.Module) -> bool:
             continue
         if isinstance(m, nn.BatchNorm2d) and not m.track_running_stats:
             continue
-        if isinstance(m, nn.LayerNorm):
+        if isinstance(m, (nn.LayerNorm, nn.GroupNorm)):
             continue
         if _broadcast_params(m) is not None:
             continue
@@ -1037,6 +1126,9 @@ def _cct_attention():
     return Attention
 
 
+_GN_ACTS = {nn.ReLU: "relu", nn.GELU: "gelu", nn.SiLU: "silu"}
+
+
 def build_template(model: nn.Module, sink: GradSink) -> nn.Module:
     memo = {id(p): p for p in model.parameters()}
     tmpl = copy.deepcopy(model, memo)
@@ -1049,6 +1141,15 @@ def build_template(model: nn.Module, sink: GradSink) -> nn.Module:
                 if type(c0) is nn.ReLU and isinstance(c1, nn.MaxPool2d):
                     setattr(mod, n0, nn.Identity())
                     setattr(mod, n1, PCMaxPool2d(c1, relu=True))
+        if type(mod) is nn.Sequential:
+            # an activation directly behind a group norm: folded into its kernel (a module that stands in several places
+            # is listed at each of them here)
+            kids = list(mod._modules.items())
+            for (n0, c0), (n1, c1) in zip(kids, kids[1:]):
+                act = _GN_ACTS.get(type(c1)) if type(c0) is nn.GroupNorm else None
+                if act is not None and getattr(c1, "approximate", "none") == "none":
+                    setattr(mod, n0, PCGroupNorm(c0, sink, act))
+                    setattr(mod, n1, nn.Identity())
         for name, child in list(mod.named_children()):
             if isinstance(child, nn.Conv2d):
                 setattr(mod, name, PCConv2d(child, sink))
@@ -1058,6 +1159,8 @@ def build_template(model: nn.Module, sink: GradSink) -> nn.Module:
                 setattr(mod, name, PCBatchNorm2d(child, sink))
             elif isinstance(child, nn.LayerNorm):
                 setattr(mod, name, PCLayerNorm(child, sink))
+            elif isinstance(child, nn.GroupNorm):
+                setattr(mod, name, PCGroupNorm(child, sink))
             elif isinstance(child, nn.MaxPool2d):
                 setattr(mod, name, PCMaxPool2d(child, relu=False))
             elif type(child) is nn.ReLU:
@@ -1109,7 +1212,7 @@ class FusedFedSGD:
         # the BatchNorm / LayerNorm backward kernels write the affine gradients before their apply pass has read the
         # affine weights — i.e. the MLP and the CNN, where the separate step is 7 % of a local step.
         self.inplace_step_ok = (_os.environ.get("BLADES_INPLACE_CLIENT_STEP", "1") != "0" and not any(
-            isinstance(m, (PCBatchNorm2d, PCLayerNorm)) for m in self.template.modules()))
+            isinstance(m, (PCBatchNorm2d, PCLayerNorm, PCGroupNorm)) for m in self.template.modules()))
         self.pc_steps_ok = 0  # completed run_per_client calls (the in-place step is taken after a first regular one)
         from blades_amd.tasks.mnist import MNIST
 

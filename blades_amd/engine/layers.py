@@ -116,6 +116,11 @@ class ClientDropout(nn.Module):
         from blades_amd import ops
 
         lay, Kc = ctx.layout, ctx.Kc
+        if x.is_cuda and lay != "single" and x.dtype in (torch.float32, torch.bfloat16, torch.float16):
+            # one kernel per pass that draws the mask where it applies it, in the backward pass again: no multipliers in
+            # memory.  (The scale is rounded to the activations' type, as a stored multiplier of that type would be.)
+            scale = ops.dropout_scale(self.p, x.dtype)
+            return ops.client_dropout(x, ctx.uids, ctx.seed, ctx.tag, self.layer, self.p, self.kind, lay, scale)
         if lay == "single":
             B = x.shape[0]
             keep = 1 if self.kind == "sample" else (2 if self.kind == "channel" and x.dim() > 2 else x.dim())

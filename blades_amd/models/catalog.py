@@ -3,7 +3,8 @@
 String dispatch is by substring like the reference — ``"cct"``, ``"resnet"``
 (= **ResNet-10**, trap noted in SURVEY), ``"mlp"``, ``"cnn"`` — with explicit
 names (``resnet18``, ``resnet34`` …, every ``cct_*``/``cvt_*`` factory) checked
-first so the north-star ResNet-18 config is expressible.
+first so the north-star ResNet-18 config is expressible.  A dict ``{"type": <explicit name>, **options}`` passes options to
+the factory (``norm: group`` of the ResNets, ``positional_embedding: rotary`` of the compact transformers).
 """
 from torch.nn import Module
 
@@ -53,6 +54,17 @@ class ModelCatalog:
             cm = model_config["custom_model"]
             cls = cm if isinstance(cm, type) else _global_registry.get(FLLIB_MODEL, cm)
             return cls(**model_config.get("custom_model_config", {}))
+        if isinstance(model_config, dict) and isinstance(model_config.get("type"), str):
+            # a named model with options: {"type": "resnet18", "norm": "group"}
+            kw = {k: v for k, v in model_config.items() if k != "type"}
+            key = model_config["type"].lower()
+            if key in _EXPLICIT:
+                return _EXPLICIT[key](**kw)
+            from . import cctnets
+
+            if key.startswith(("cct_", "cvt_")) and hasattr(cctnets, key):
+                return getattr(cctnets, key)(**kw)
+            raise NotImplementedError(f"Unknown model type `{model_config['type']}` (options need an explicit name)")
         raise NotImplementedError(f"Cannot build a model from {model_config!r}")
 
     @staticmethod

@@ -4,6 +4,8 @@ Factory names follow Compact-Transformers / the reference (``fllib/models/backbo
 ``cct_<L>_<k>x<n>_<img>[_sine][_c100]`` — L encoder layers, n conv layers of kernel k, image size —
 and ``cvt_<L>_<patch>_<img>[_sine]``.  Only ``cct_2_3x2_32`` is reachable through the reference's
 model catalog (``global_model: cct``); all the others are addressable here by their full name.
+``positional_embedding="rotary"`` (any factory) turns queries and keys by their patch's row and column instead of adding a
+table to the tokens.
 No pretrained weights are downloadable offline: ``pretrained=True`` raises.
 """
 from functools import partial
@@ -29,7 +31,8 @@ class CCT(nn.Module):
         self.classifier = TransformerClassifier(
             True, embedding_dim, num_layers, num_heads, mlp_ratio, num_classes, dropout, attention_dropout,
             stochastic_depth, positional_embedding,
-            self.tokenizer.sequence_length(n_input_channels, img_size, img_size))
+            self.tokenizer.sequence_length(n_input_channels, img_size, img_size),
+            self.tokenizer.grid(n_input_channels, img_size, img_size) if positional_embedding == "rotary" else None)
 
     def forward(self, x):
         return self.classifier(self.tokenizer(x))
@@ -46,7 +49,8 @@ class CVT(nn.Module):
         self.classifier = TransformerClassifier(
             True, embedding_dim, num_layers, num_heads, mlp_ratio, num_classes, dropout, attention_dropout,
             stochastic_depth, positional_embedding,
-            self.tokenizer.sequence_length(n_input_channels, img_size, img_size))
+            self.tokenizer.sequence_length(n_input_channels, img_size, img_size),
+            self.tokenizer.grid(n_input_channels, img_size, img_size) if positional_embedding == "rotary" else None)
 
     def forward(self, x):
         return self.classifier(self.tokenizer(x))

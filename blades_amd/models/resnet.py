@@ -9,7 +9,12 @@ batch, i.e. statistics are per (client, channel).
 Parameter names (conv1, bn1, layer{1..4}.{i}.conv1/bn1/conv2/bn2/shortcut.0/1,
 linear) and their order match the reference, so D and the flattening agree:
 ResNet10 D = 4,903,242, ResNet18 D = 11,173,962.
+
+``norm="group"`` puts a GroupNorm of ``norm_groups`` groups in every BatchNorm's place (same names, same D): a sample's
+output then does not depend on the rest of its batch, which is what clients with differing data, and differential
+privacy, ask for.
 """
+from functools import partial
 from typing import Sequence
 
 import torch.nn.functional as F
@@ -20,22 +25,30 @@ def _bn(c):
     return nn.BatchNorm2d(c, track_running_stats=False)
 
 
-def _shortcut(cin, cout, stride):
+def _norm(kind: str, groups: int):
+    if kind == "batch":
+        return _bn
+    if kind == "group":
+        return partial(nn.GroupNorm, groups)
+    raise ValueError(f"norm must be 'batch' or 'group', got {kind!r}")
+
+
+def _shortcut(cin, cout, stride, norm=_bn):
     if stride == 1 and cin == cout:
         return nn.Sequential()
-    return nn.Sequential(nn.Conv2d(cin, cout, 1, stride=stride, bias=False), _bn(cout))
+    return nn.Sequential(nn.Conv2d(cin, cout, 1, stride=stride, bias=False), norm(cout))
 
 
 class BasicBlock(nn.Module):
     expansion = 1
 
-    def __init__(self, in_planes, planes, stride=1):
+    def __init__(self, in_planes, planes, stride=1, norm=_bn):
         super().__init__()
         self.conv1 = nn.Conv2d(in_planes, planes, 3, stride=stride, padding=1, bias=False)
-        self.bn1 = _bn(planes)
+        self.bn1 = norm(planes)
         self.conv2 = nn.Conv2d(planes, planes, 3, stride=1, padding=1, bias=False)
-        self.bn2 = _bn(planes)
-        self.shortcut = _shortcut(in_planes, planes * self.expansion, stride)
+        self.bn2 = norm(planes)
+        self.shortcut = _shortcut(in_planes, planes * self.expansion, stride, norm)
 
     def forward(self, x):
         out = F.relu(self.bn1(self.conv1(x)))
@@ -46,15 +59,15 @@ class BasicBlock(nn.Module):
 class Bottleneck(nn.Module):
     expansion = 4
 
-    def __init__(self, in_planes, planes, stride=1):
+    def __init__(self, in_planes, planes, stride=1, norm=_bn):
         super().__init__()
         self.conv1 = nn.Conv2d(in_planes, planes, 1, bias=False)
-        self.bn1 = _bn(planes)
+        self.bn1 = norm(planes)
         self.conv2 = nn.Conv2d(planes, planes, 3, stride=stride, padding=1, bias=False)
-        self.bn2 = _bn(planes)
+        self.bn2 = norm(planes)
         self.conv3 = nn.Conv2d(planes, planes * self.expansion, 1, bias=False)
-        self.bn3 = _bn(planes * self.expansion)
-        self.shortcut = _shortcut(in_planes, planes * self.expansion, stride)
+        self.bn3 = norm(planes * self.expansion)
+        self.shortcut = _shortcut(in_planes, planes * self.expansion, stride, norm)
 
     def forward(self, x):
         out = F.relu(self.bn1(self.conv1(x)))
@@ -64,21 +77,23 @@ class Bottleneck(nn.Module):
 
 
 class ResNet(nn.Module):
-    def __init__(self, block, num_blocks: Sequence[int], num_classes: int = 10, in_channels: int = 3):
+    def __init__(self, block, num_blocks: Sequence[int], num_classes: int = 10, in_channels: int = 3,
+                 norm: str = "batch", norm_groups: int = 32):
         super().__init__()
         self.in_planes = 64
+        make_norm = _norm(norm, norm_groups)
         self.conv1 = nn.Conv2d(in_channels, 64, 3, stride=1, padding=1, bias=False)
-        self.bn1 = _bn(64)
-        self.layer1 = self._stage(block, 64, num_blocks[0], 1)
-        self.layer2 = self._stage(block, 128, num_blocks[1], 2)
-        self.layer3 = self._stage(block, 256, num_blocks[2], 2)
-        self.layer4 = self._stage(block, 512, num_blocks[3], 2)
+        self.bn1 = make_norm(64)
+        self.layer1 = self._stage(block, 64, num_blocks[0], 1, make_norm)
+        self.layer2 = self._stage(block, 128, num_blocks[1], 2, make_norm)
+        self.layer3 = self._stage(block, 256, num_blocks[2], 2, make_norm)
+        self.layer4 = self._stage(block, 512, num_blocks[3], 2, make_norm)
         self.linear = nn.Linear(512 * block.expansion, num_classes)
 
-    def _stage(self, block, planes, n, stride):
+    def _stage(self, block, planes, n, stride, norm):
         blocks = []
         for s in [stride] + [1] * (n - 1):
-            blocks.append(block(self.in_planes, planes, s))
+            blocks.append(block(self.in_planes, planes, s, norm))
             self.in_planes = planes * block.expansion
         return nn.Sequential(*blocks)
 

@@ -7,6 +7,8 @@ raises.  CPU tensors run ``reference.py`` (the numerical contract the kernels
 are tested against), which is what keeps the whole framework runnable and
 testable on a machine without a GPU.
 """
+import functools
+
 import torch
 
 from . import reference as ref
@@ -291,6 +293,13 @@ def client_dropout_mult(uids, n, seed, tag, layer, p):
             and not torch._C._functorch.is_batchedtensor(uids):
         return _h().client_dropout_mult(uids, int(n), int(seed), tag, int(layer), float(p))
     return ref.client_dropout_mult(uids, n, seed, tag, layer, p)
+
+
+@functools.lru_cache(maxsize=256)
+def dropout_scale(p, dtype=torch.float32):
+    """Scale of kept elements, 1 / (1 - p) in 32 bits, rounded to ``dtype``."""
+    one = torch.ones((), dtype=torch.float32)
+    return float((one / (one - torch.tensor(p, dtype=torch.float32))).to(dtype))
 
 
 from .layers import client_dropout, group_norm, rope_axes  # noqa: E402,F401 — differentiable, see layers.py
