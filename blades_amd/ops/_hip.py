@@ -1800,6 +1800,25 @@ _rope_plan_size = _opt_sig("blades_rope_plan_size", [], c_long)
 _rope_plan_fill = _opt_sig("blades_rope_plan", [_P, c_int, c_long, c_long, c_long, c_int, c_int, c_int, c_long, c_long, c_long,
                                                 c_long, c_int, _P, c_int, c_double, c_int, c_int], c_int)
 _rope = _opt_sig("blades_rope_axes", [_P, _P, _P, _P, c_int, _P], c_int)
+_autograd = None
+
+
+def autograd():
+    """The C++ autograd nodes (csrc/autograd.cpp), bound to this library's entry points."""
+    global _autograd
+    if _autograd is None:
+        if not _build.AUTOGRAD_LIB.exists():
+            raise ImportError(f"{_build.AUTOGRAD_LIB} is missing: build it with `python -m blades_amd.ops.build`. GPU tensors "
+                              "have no other implementation.")
+        import importlib
+
+        m = importlib.import_module("blades_amd.ops._autograd")
+        m.entries([ctypes.cast(f, c_void_p).value for f in (_gn_plan_size, _gn_plan_fill, _gn_fwd, _gn_bwd, _client_drop,
+                                                            _rope_plan_size, _rope_plan_fill, _rope)])
+        _autograd = m
+    return _autograd
+
+
 _raw_stream, _device_now = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 

@@ -6,6 +6,10 @@
 Both expose a plain C ABI and are loaded with ctypes, so neither needs the
 PyTorch headers: a full rebuild is seconds, and hipcc cross-compiles gfx950
 code objects on a machine without a GPU.
+
+* ``_autograd.so``       — g++, ``csrc/autograd.cpp`` (no device code): the autograd
+  nodes of ``ops/layers.py``, the one file that includes PyTorch's headers; it calls
+  ``libblades_hip.so`` through addresses
 """
 import os
 import re
@@ -17,6 +21,7 @@ HERE = Path(__file__).resolve().parent
 CSRC = HERE / "csrc"
 HOST_LIB = HERE / "libblades_host.so"
 HIP_LIB = HERE / "libblades_hip.so"
+AUTOGRAD_LIB = HERE / "_autograd.so"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 # scalar fp32 instructions only: some forms of the packed ones (v_pk_fma_f32 and its like), which -O3 makes of ordinary
@@ -87,9 +92,31 @@ def build_hip(force: bool = False, verbose: bool = False, jobs: int = 4) -> Path
     return HIP_LIB
 
 
+def build_autograd(force: bool = False, verbose: bool = False) -> Path:
+    src = CSRC / "autograd.cpp"
+    if force or _stale(AUTOGRAD_LIB, [src]):
+        import sysconfig
+
+        import torch
+        from torch.utils.cpp_extension import include_paths
+
+        lib = Path(torch.__file__).parent / "lib"
+        rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+        inc = include_paths() + [f"{rocm}/include", sysconfig.get_paths()["include"]]
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+               "-DTORCH_EXTENSION_NAME=_autograd", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+        cmd += [a for i in inc for a in ("-isystem", i)] + [str(src), "-o", str(AUTOGRAD_LIB), f"-L{lib}", "-ltorch",
+                                                            "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip"]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.check_call(cmd)
+    return AUTOGRAD_LIB
+
+
 def build_all(force: bool = False, verbose: bool = True):
     build_host(force, verbose)
     build_hip(force, verbose)
+    build_autograd(force, verbose)
 
 
 if __name__ == "__main__":

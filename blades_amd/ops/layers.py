@@ -10,30 +10,33 @@
 
 CUDA tensors run the hand-written kernels (fp32, bf16 or fp16; anything else raises), CPU tensors and tensors wrapped by
 ``torch.func`` transforms the oracles of ``reference.py``.  Arguments are checked alike on both.  The gradients are
-first-order: a second backward pass raises.
+first-order: differentiating them again raises.  The autograd nodes are C++ (csrc/autograd.cpp): both passes run without
+the interpreter.
 """
+import functools
+import math
+from ctypes import c_float
+
 import torch
-from torch.autograd.function import once_differentiable
 
 import blades_amd.ops as _ops
 
 from . import reference as ref
 
-_ACTS = ("none", "relu", "gelu", "silu")
+_ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 _KINDS = ("elem", "channel", "sample")
 _P_END = 1.0 - 2.0 ** -25  # rounds to 1 in 32 bits from here
 _POS = (torch.int64, torch.float32)
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _wrapped = torch._C._functorch.is_functorch_wrapped_tensor
-_grad_mode = torch.is_grad_enabled
-_kernels = None
+_loaded = None
 
 
-def _h():
-    global _kernels
-    if _kernels is None:
-        _kernels = _ops._h()
-    return _kernels
+def _nodes():
+    global _loaded
+    if _loaded is None:
+        _loaded = _ops._h().autograd()
+    return _loaded
 
 
 def _own_kernel(name: str, t: torch.Tensor) -> bool:
@@ -42,74 +45,6 @@ def _own_kernel(name: str, t: torch.Tensor) -> bool:
     if t.dtype not in _DTYPES:
         raise ValueError(f"{name}: CUDA tensors must be fp32, bf16 or fp16, got {t.dtype}")
     return True
-
-
-def _first_order(backward):
-    """A backward that must not be differentiated again.  torch's wrapper for that costs 6 us a call; it is only needed
-    while a graph of the backward pass is being built."""
-    guarded = once_differentiable(backward)
-
-    def call(ctx, gy):
-        return guarded(ctx, gy) if _grad_mode() else backward(ctx, gy)
-
-    return call
-
-
-class _GroupNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, residual, cfg):
-        groups, eps, act = cfg
-        w, b = _affine(weight), _affine(bias)
-        clients = _clients(w, b)
-        y, stats, gate, plan = _h().group_norm_forward(x, groups, w, b, eps, act, residual, clients, True, True)
-        lead = None  # the types of affine vectors that are not fp32
-        if w is not None and weight.dtype != w.dtype or b is not None and bias.dtype != b.dtype:
-            lead = (None if weight is None else weight.dtype, None if bias is None else bias.dtype)
-        ctx.cfg = (groups, act, clients, plan, lead)
-        # the gate stands in for the residual; without one z is computed again, from x and a smooth activation's residual
-        ctx.save_for_backward(x, w, b, stats, residual if act in ("gelu", "silu") else None, gate)
-        return y
-
-    @staticmethod
-    @_first_order
-    def backward(ctx, gy):
-        x, w, b, stats, res, gate = ctx.saved_tensors
-        groups, act, clients, plan, lead = ctx.cfg
-        nx, nw, nb, nr, _ = ctx.needs_input_grad
-        dw = torch.empty(w.shape, device=x.device) if nw else None
-        db = torch.empty(b.shape, device=x.device) if nb else None
-        dx, dres = _kernels.group_norm_backward(x, gy, groups, w, b, stats, plan, act, res, gate, clients, nx,
-                                                nr and act != "none", dw, db, x.shape[1], None, False, True)
-        if nr and act == "none":
-            dres = gy
-        if lead is not None:
-            dw = dw if dw is None else dw.to(lead[0])
-            db = db if db is None else db.to(lead[1])
-        return dx, dw, db, dres, None
-
-
-def _affine(t):
-    if t is None:
-        return None
-    t = t.detach()
-    if t.dtype != torch.float32:
-        t = t.to(torch.float32)
-    return t if t.stride(-1) == 1 else t.contiguous()
-
-
-def _clients(*affine):
-    for t in affine:
-        if t is not None and t.dim() == 2:
-            return t.shape[0]
-    return 1
-
-
-def _needs_grad(*tensors) -> bool:
-    if _grad_mode():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
-    return False
 
 
 def group_norm(x, groups: int, weight=None, bias=None, eps: float = 1e-5, act: str = "none", residual=None):
@@ -126,7 +61,7 @@ def group_norm(x, groups: int, weight=None, bias=None, eps: float = 1e-5, act: s
     if groups < 1 or C < 1 or C % groups:
         raise ValueError(f"group_norm: {C} channels do not divide into {groups} groups")
     if act not in _ACTS:
-        raise ValueError(f"group_norm: act must be one of {_ACTS}, got {act!r}")
+        raise ValueError(f"group_norm: act must be one of {tuple(_ACTS)}, got {act!r}")
     if not eps >= 0.0:
         raise ValueError(f"group_norm: eps must not be negative, got {eps}")
     for t in (weight, bias):
@@ -144,37 +79,7 @@ def group_norm(x, groups: int, weight=None, bias=None, eps: float = 1e-5, act: s
                          f"{tuple(residual.shape)} on {residual.device}")
     if not _own_kernel("group_norm", x) or x.numel() == 0:
         return ref.group_norm(x, groups, weight, bias, eps, act, residual)
-    if _needs_grad(x, weight, bias, residual):
-        return _GroupNormFn.apply(x, weight, bias, residual, (groups, eps, act))
-    w, b = _affine(weight), _affine(bias)
-    return _h().group_norm_forward(x, groups, w, b, eps, act, residual, _clients(w, b), False, True)[0]
-
-
-class _ClientDropoutFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, uids, tag, cfg):
-        h = _h()
-        x, plan = h.dropout_plan(x, uids, *cfg)
-        # the ids and the tag are saved, so that changing them between the two passes raises instead of drawing another mask
-        if type(tag) is int:
-            ctx.save_for_backward(uids)
-            ctx.run = (plan, x.stride(), cfg, tag)
-        else:
-            ctx.save_for_backward(uids, tag)
-            ctx.run = (plan, x.stride(), cfg, None)
-        return h.dropout_launch(x, uids, tag, plan)
-
-    @staticmethod
-    @_first_order
-    def backward(ctx, gy):
-        plan, stride, cfg, tag = ctx.run
-        if tag is None:
-            uids, tag = ctx.saved_tensors
-        else:
-            (uids,) = ctx.saved_tensors
-        if gy.stride() != stride:
-            gy, plan = _h().dropout_plan(gy, uids, *cfg)
-        return _kernels.dropout_launch(gy, uids, tag, plan), None, None, None
+    return _nodes().group_norm(x, groups, weight, bias, eps, _ACTS[act], residual)
 
 
 def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "elem", layout: str = "major", scale=None):
@@ -207,28 +112,20 @@ def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "e
         return x.clone()
     if not _own_kernel("client_dropout", x):
         return ref.client_dropout(x, uids, seed, tag, layer, p, kind, layout, scale)
-    cfg = (int(seed), int(layer), p, kind, layout, None if scale is None else float(scale))  # (dropout_plan's)
     if uids.dim() == 0 or not uids.is_contiguous():
         uids = uids.reshape(-1).contiguous()
-    if by_value:
-        tag = int(tag)
-    if x.requires_grad and _grad_mode():
-        return _ClientDropoutFn.apply(x, uids, tag, cfg)
-    x, plan = _h().dropout_plan(x, uids, *cfg)
-    return _kernels.dropout_launch(x, uids, tag, plan)
+    least, times = _draw(p)
+    code = 0 if kind == "elem" or (kind == "channel" and x.dim() <= 2) else 1 if kind == "channel" else 2
+    return _nodes().client_dropout(x, uids, None if by_value else tag, int(tag) & 0xFFFFFFFF if by_value else 0, int(seed) & (2 ** 64 - 1),
+                                   (2 + 256 * int(layer)) & 0xFFFFFFFF, least, times if scale is None else float(scale), code,
+                                   inner)
 
 
-class _RopeFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, pos, cfg):
-        ctx.save_for_backward(pos)
-        ctx.cfg = cfg
-        return _h().rope_axes(x, pos, *cfg, False, None, True)
-
-    @staticmethod
-    @_first_order
-    def backward(ctx, gy):
-        return _h().rope_axes(gy, ctx.saved_tensors[0], *ctx.cfg, True, None, True), None, None
+@functools.lru_cache(maxsize=256)
+def _draw(p: float):
+    """(smallest 24-bit draw that is kept, 1 / (1 - p)), both in 32 bits."""
+    p32 = c_float(p).value
+    return math.ceil(p32 * 16777216.0), c_float(1.0 / c_float(1.0 - p32).value).value
 
 
 def rope_axes(x, pos, axes, base: float = 10000.0, slots=None):
@@ -259,6 +156,4 @@ def rope_axes(x, pos, axes, base: float = 10000.0, slots=None):
                          f"{len(axes)}] on {x.device} without a gradient, got {pos.dtype} {tuple(shape)} on {pos.device}")
     if not _own_kernel("rope_axes", x):
         return ref.rope_axes(x, pos, axes, base, slots)
-    if x.requires_grad and _grad_mode():
-        return _RopeFn.apply(x, pos, (axes, base, slots))
-    return _h().rope_axes(x, pos, axes, base, slots, False, None, True)
+    return _nodes().rope_axes(x, pos, axes, base, slots)
