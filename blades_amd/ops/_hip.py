@@ -12,7 +12,6 @@ fall back to a PyTorch implementation.
 import ctypes
 import functools
 from ctypes import c_double, c_float, c_int, c_long, c_uint, c_ulonglong, c_void_p
-from math import ceil as _ceil
 from typing import Optional
 
 import torch
@@ -1984,76 +1983,6 @@ def group_norm_backward(x, gy, groups: int, weight, bias, stats, plan, act: str 
             stats.data_ptr(), _dp(dx), _dp(dres), _dp(coef), _dp(dweight), _dp(dbias), ld, int(accumulate), ws.data_ptr(),
             plan.at)
     return dx, dres
-
-
-def dropout_scale(p: float) -> float:
-    """1 / (1 - p) as the kernels compute it: in 32 bits."""
-    q = c_float(1.0 - c_float(p).value).value
-    return c_float(1.0 / q).value
-
-
-class _DropPlan(ctypes.Structure):
-    _fields_ = [("B", c_long), ("C", c_long), ("HW", c_long), ("seed", c_ulonglong), ("Kc", c_int), ("kind", c_int),
-                ("inner", c_int), ("last", c_int), ("dtype", c_int), ("c3", c_uint), ("least", c_uint), ("scale", c_float)]
-
-
-@functools.lru_cache(maxsize=4096)
-def _drop_plan(shape, Kc, last, dtype, seed, layer, p, kind, layout, scale):
-    """(plan, its address): what a client_dropout launch's shape and key fix."""
-    if layout == "major":
-        B, C = shape[0] // Kc, (shape[1] if len(shape) > 1 else 1)
-    else:
-        B, C = shape[0], shape[1] // Kc
-    numel = 1
-    for d in shape:
-        numel *= d
-    if numel // Kc > 17e9:
-        raise ValueError("client_dropout: a client's share of a layer has at most 1.7e10 elements")
-    plan = _DropPlan(B, C, numel // (Kc * B * C), seed & (2 ** 64 - 1), Kc,
-                     {"elem": 0, "channel": 1 if len(shape) > 2 else 0, "sample": 2}[kind], layout == "inner", last,
-                     _DT_CODE[dtype], (2 + 256 * layer) & 0xFFFFFFFF, _ceil(c_float(p).value * 16777216.0),
-                     dropout_scale(p) if scale is None else scale)
-    return plan, ctypes.addressof(plan)
-
-
-def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "elem", layout: str = "major", scale=None,
-                   checked: bool = False):
-    """``x`` times its client-keyed dropout multipliers (see reference.client_dropout), nothing stored.  ``tag``: an int,
-    or a 1-element int64 tensor read when the kernel runs (captured graphs).  ``checked``: the caller did."""
-    if not checked:
-        if not (x.is_cuda and x.dtype in _DT_CODE and x.dim() >= 1):
-            raise ValueError(f"client_dropout: expected a CUDA fp32 / bf16 / fp16 tensor, got {x.device} {x.dtype}")
-        if not (uids.device == x.device and uids.dtype == torch.int64 and uids.dim() == 1 and uids.is_contiguous()
-                and uids.numel() > 0 and x.shape[1 if layout == "inner" else 0] % uids.numel() == 0):
-            raise ValueError("client_dropout: uids must be a contiguous int64 vector on x's device that divides the batch")
-        if torch.is_tensor(tag) and not (tag.device == x.device and tag.dtype == torch.int64 and tag.numel() == 1):
-            raise ValueError("client_dropout: tag must be an int or a 1-element int64 tensor on x's device")
-        tag = tag if torch.is_tensor(tag) else int(tag)
-        if not 0.0 <= c_float(p).value < 1.0:
-            raise ValueError("client_dropout: need 0 <= p < 1 in 32 bits")
-    if x.numel() == 0:
-        return x.clone()
-    x, plan = dropout_plan(x, uids, seed, layer, p, kind, layout, scale)
-    return dropout_launch(x, uids, tag, plan)
-
-
-def dropout_plan(x, uids, seed, layer, p, kind, layout, scale):
-    """(x as the kernel takes it, plan)."""
-    last = False
-    if not x.is_contiguous():
-        last = x.dim() == 4 and x.is_contiguous(memory_format=torch.channels_last)
-        x = x if last else x.contiguous()
-    return x, _drop_plan(x.shape, uids.numel(), last, x.dtype, seed, layer, p, kind, layout, scale)
-
-
-def dropout_launch(x, uids, tag, plan):
-    """The plan's dropout of a tensor that lies as the one the plan was made for.  ``tag``: int, or tensor."""
-    y = _empty_like(x)
-    value, at = (tag, None) if type(tag) is int else (0, tag.data_ptr())
-    rc = _launch(x.device.index, _client_drop, x.data_ptr(), y.data_ptr(), uids.data_ptr(), at, value, plan[1])
-    if rc != 0:
-        raise ValueError(f"client_dropout: rejected (rc={rc})")
-    return y
 
 
 @functools.lru_cache(maxsize=4096)

@@ -207,48 +207,32 @@ __global__ __launch_bounds__(MAX_THREADS) void gn_bwd_chunk_kernel(Geo q, const 
     part[((size_t)w.n * q.nchunk + w.chunk) * q.C + w.slab * q.S + c] = make_float2(ch[c], ch[q.S + c]);
 }
 
-// Joins the chunks' (A, B): channel sums of a sample (for the affine gradients) and gamma times them, 16 channels x 16
-// parts of the chunks a workgroup, fixed order; then the group means for the second sweep, one wave per (sample, group).
-constexpr int JOIN_CH = 16, JOIN_PARTS = 16;
-__global__ __launch_bounds__(JOIN_CH * JOIN_PARTS) void gn_bwd_join_kernel(const float2* __restrict__ part, int n0, int C,
-                                                                          int nchunk, float2* __restrict__ sums) {
-  __shared__ double red[JOIN_PARTS][JOIN_CH][2];
-  const int groups = (C + JOIN_CH - 1) / JOIN_CH, i = blockIdx.x / groups;
-  const int cl = threadIdx.x % JOIN_CH, r = threadIdx.x / JOIN_CH, c = (blockIdx.x - i * groups) * JOIN_CH + cl;
-  double a = 0.0, b = 0.0;
-  if (c < C)
-    for (int k = r; k < nchunk; k += JOIN_PARTS) {
-      const float2 e = part[((size_t)i * nchunk + k) * C + c];
-      a += (double)e.x; b += (double)e.y;
-    }
-  red[r][cl][0] = a; red[r][cl][1] = b;
-  __syncthreads();
-  if (r != 0 || c >= C) return;
-#pragma unroll
-  for (int k = 1; k < JOIN_PARTS; ++k) { a += red[k][cl][0]; b += red[k][cl][1]; }
-  sums[(size_t)(n0 + i) * C + c] = make_float2((float)a, (float)b);
-}
-__global__ __launch_bounds__(256) void gn_bwd_means_kernel(const float2* __restrict__ sums, int n0, int cnt, int C, int D, int P,
-                                                           int per_client, const float* __restrict__ gamma, long gstride,
-                                                           float2* __restrict__ means) {
+// The group means of the second sweep from the chunks' (A, B): one wave per (sample, group), fixed order.
+__global__ __launch_bounds__(256) void gn_bwd_means_kernel(const float2* __restrict__ part, int n0, int cnt, int C, int D, int P,
+                                                           int nchunk, int per_client, const float* __restrict__ gamma,
+                                                           long gstride, float2* __restrict__ means) {
   const int G = C / D, lane = threadIdx.x & 63;
   const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (i >= (long)cnt * G) return;
-  const long n = n0 + i / G;
-  const int g = (int)(i % G);
+  const long n = i / G;
+  const int g = (int)(i - n * G);
+  const float* gam = gamma ? gamma + ((n0 + n) / per_client) * gstride + g * D : nullptr;
+  const float2* p = part + (size_t)n * nchunk * C + g * D;
   double a = 0.0, b = 0.0;
-  for (int c = g * D + lane; c < (g + 1) * D; c += 64) {
-    const float w = gamma ? gamma[(n / per_client) * gstride + c] : 1.f;
-    const float2 e = sums[(size_t)n * C + c];
+  for (long j = lane; j < (long)nchunk * D; j += 64) {
+    const long k = j / D;
+    const int d = (int)(j - k * D);
+    const float w = gam ? gam[d] : 1.f;
+    const float2 e = p[k * C + d];
     a += (double)w * e.x; b += (double)w * e.y;
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); b += __shfl_xor(b, o, 64); }
   const double inv = 1.0 / ((double)P * D);
-  if (lane == 0) means[(size_t)n * G + g] = make_float2((float)(a * inv), (float)(b * inv));
+  if (lane == 0) means[i] = make_float2((float)(a * inv), (float)(b * inv));
 }
 
-// dgamma / dbeta of a client: its samples' (A, B), 8 channels x 128 rows of threads a workgroup, fixed order
+// dgamma / dbeta of a client: the (A, B) of its `per_client` rows (samples, or samples' chunks), 8 channels x 128 rows of threads a workgroup, fixed order
 constexpr int AFF_CH = 8, AFF_ROWS = 128;
 __global__ __launch_bounds__(AFF_CH * AFF_ROWS) void gn_affine_kernel(const float2* __restrict__ sums, int per_client, int C,
                                                                       const float* __restrict__ coef, float* __restrict__ dg,
@@ -282,9 +266,8 @@ int backward_t(const Plan& pl, const void* x, const void* res, const void* gy, c
                const float* beta, const float* mean, const float* rstd, void* dx, void* dres, float* ws, hipStream_t st) {
   const Geo& q = pl.q;
   const int G = q.C / q.D, N = q.N;
-  float2* sums = (float2*)ws;              // [N][C]
-  float2* means = sums + (size_t)N * q.C;  // [N][G]               (these two: split plans alone)
-  float2* part = means + (size_t)N * G;    // [piece][nchunk][C]
+  float2* sums = (float2*)ws;                                         // [N][nchunk][C]
+  float2* means = sums + (size_t)N * q.nchunk * q.C;                  // [piece][G], split plans alone
   const size_t per = (size_t)q.P * q.C;
   for (long n0 = 0; n0 < N; n0 += pl.piece) {
     Geo s = q;
@@ -295,22 +278,21 @@ int backward_t(const Plan& pl, const void* x, const void* res, const void* gy, c
     T *dp = dx ? (T*)dx + n0 * per : nullptr, *ep = dres ? (T*)dres + n0 * per : nullptr;
     const float *mp = mean + n0 * G, *sp = rstd + n0 * G;
     const dim3 grid((unsigned)((s.N + 7) / 8 * 8) * q.nslab * q.nchunk), block(pl.threads);
+    float2* part = sums + (size_t)n0 * q.nchunk * q.C;
     if (pl.split) {
-      hipLaunchKernelGGL((gn_bwd_chunk_kernel<T, VEC, NM, AK, false>), grid, block, pl.lds, st, s, xp, rp, gp, tp, gamma, beta, mp,
-                         sp, (T*)nullptr, (T*)nullptr, part, (const float2*)nullptr);
-      hipLaunchKernelGGL(gn_bwd_join_kernel, dim3((unsigned)s.N * cdiv(q.C, JOIN_CH)), dim3(JOIN_CH * JOIN_PARTS), 0, st,
-                         (const float2*)part, (int)n0, q.C, q.nchunk, sums);
+      hipLaunchKernelGGL((gn_bwd_chunk_kernel<T, VEC, NM, AK, false>), grid, block, pl.lds, st, s, xp, rp, gp, tp, gamma, beta,
+                         mp, sp, (T*)nullptr, (T*)nullptr, part, (const float2*)nullptr);
       if (dx == nullptr && dres == nullptr) continue;
-      hipLaunchKernelGGL(gn_bwd_means_kernel, dim3(cdiv((long)s.N * G, 4)), dim3(256), 0, st, (const float2*)sums, (int)n0, s.N,
-                         q.C, q.D, q.P, q.per_client, gamma, q.gstride, means);
+      hipLaunchKernelGGL(gn_bwd_means_kernel, dim3(cdiv((long)s.N * G, 4)), dim3(256), 0, st, (const float2*)part, (int)n0, s.N,
+                         q.C, q.D, q.P, q.nchunk, q.per_client, gamma, q.gstride, means);
       s.back = 1;
-      hipLaunchKernelGGL((gn_bwd_chunk_kernel<T, VEC, NM, AK, true>), grid, block, 0, st, s, xp, rp, gp, tp, gamma, beta, mp, sp, dp,
-                         ep, (float2*)nullptr, (const float2*)(means + n0 * G));
+      hipLaunchKernelGGL((gn_bwd_chunk_kernel<T, VEC, NM, AK, true>), grid, block, 0, st, s, xp, rp, gp, tp, gamma, beta, mp, sp,
+                         dp, ep, (float2*)nullptr, (const float2*)means);
       continue;
     }
 #define GN_BWD(RR)                                                                                                         \
   hipLaunchKernelGGL((gn_bwd_kernel<T, VEC, RR, NM, AK>), grid, block, pl.lds, st, s, xp, rp, gp, tp, gamma, beta, mp, sp, dp, \
-                     ep, sums + n0 * q.C)
+                     ep, part)
     switch (pl.R) {
       case 1: case 2: case 4: GN_BWD(4); break;
       case 8: GN_BWD(8); break;
@@ -348,11 +330,13 @@ BLADES_API int blades_group_norm_backward(const void* x, const void* res, const 
 #undef GN_B
   if (dgamma != nullptr || dbeta != nullptr) {
     const int groups = cdiv(q.C, AFF_CH);
+    const long rows = (long)q.per_client * q.nchunk;
+    if (rows >= (1L << 31)) return 1;
     const long clients = q.N / q.per_client, most = ((1L << 32) - 1) / ((long)groups * AFF_CH * AFF_ROWS);
     for (long k = 0; k < clients; k += most) {
       const long n = clients - k < most ? clients - k : most;
       hipLaunchKernelGGL(gn_affine_kernel, dim3((unsigned)(n * groups)), dim3(AFF_CH * AFF_ROWS), 0, st,
-                         (const float2*)ws + k * q.per_client * q.C, q.per_client, q.C, coef ? coef + k : nullptr,
+                         (const float2*)ws + k * rows * q.C, (int)rows, q.C, coef ? coef + k : nullptr,
                          dgamma ? dgamma + k * ld : nullptr, dbeta ? dbeta + k * ld : nullptr, ld, accumulate);
     }
   }

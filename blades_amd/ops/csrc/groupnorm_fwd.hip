@@ -270,7 +270,7 @@ BLADES_API int blades_group_norm_plan(Layer* p, long N, long P, int C, int G, fl
     if (!make_plan(pl, N, P, C, G, dtype == 0 ? 4 : 2, vec, k + 1, per_client)) return 2;
     pl.q.eps = eps; pl.q.act = act; pl.q.gstride = gstride; pl.q.bstride = bstride;
     pl.ws = k == 0 ? (pl.split ? pl.piece * pl.q.nchunk * G * 8 : 0)
-                   : (N * C + (pl.split ? N * G + pl.piece * pl.q.nchunk * C : 0)) * 8;
+                   : (N * pl.q.nchunk * C + (pl.split ? pl.piece * G : 0)) * 8;
     ws[k] = pl.ws;
   }
   return 0;
