@@ -11,11 +11,17 @@
 // A workgroup takes a slab: the S = k * D channels of whole groups of one sample, all pixels, held in registers (up to
 // 64 values a thread), so x is read from memory once in each direction: mean, then the squares around that mean (no
 // cancellation for offset activations), then the result, all from registers.  Lane l of a pixel row owns VEC channels
-// (16 bytes), so a thread keeps its channels for the whole sweep.  A sample too large for a workgroup's registers is
+// (four, or one where the channel count or an address does not allow it), so a thread keeps its channels for the whole sweep.
+// A sample too large for a workgroup's registers is
 // cut into pixel chunks: a first sweep leaves (mean, M2) or (A, B) of each, a small kernel joins them in chunk order, and a
 // second sweep applies, from the last sample to the first: what the first sweep read last is still in the 256 MB cache
 // (walking the batch in pieces that fit it as a whole costs more in launches than it saves: 48 x 64 x 112 x 112 fp32
-// forward + backward 380 us in pieces of 96 MB, 319 in 180 MB, 292 at once).  All sums are fp32 in a fixed order (double where many partial sums meet): bitwise reproducible.
+// forward + backward 380 us in pieces of 96 MB, 319 in 180 MB, 292 at once).  All sums are fp32 in a fixed order (double
+// where many partial sums meet): bitwise reproducible.
+//
+// Bound by memory.  Measured (MI355X; copies run at 5.0 - 5.4 TB/s beyond the last-level cache, at 8 within it): 2048 x 64 x
+// 32 x 32 fp32 forward 198 us (5.4 TB/s), backward 320 (5.0); 2048 x 128 x 16 x 16 bf16 SiLU 47 and 80 (5.7, 5.0); 2048 x 512
+// x 4 x 4 fp32 with a residual 32 and 54 (6.4, 5.2); two sweeps of 48 x 64 x 112 x 112 fp32 27 + 48 and 52 + 72 (5.9).
 #pragma once
 #include "common.h"
 
@@ -37,7 +43,6 @@ constexpr int MAX_THREADS = 1024;  // of 128 registers
 constexpr int BLOCK = 4;           // vectors a thread has in flight in the sweeps over pixel chunks
 // channels of a slab with several groups, and of a single group: the backward pass's sums then fit 64 KB of LDS
 constexpr int MAX_SLAB = 1024, MAX_GROUP = 2048;
-
 
 struct Geo {
   int N, P, C, D;                    // samples of this launch, pixels, channels, channels of a group
@@ -259,17 +264,18 @@ inline bool make_plan(Plan& pl, long N, long P, int C, int G, int esize, int vec
   q.tw_gr = team(D);
   pl.lds = hold == 1 ? (2 * (size_t)Gs + (size_t)nr * q.L * nm) * 4
                      : (3 * (size_t)q.S + 4 * (size_t)Gs + 2 * (size_t)nr * q.S) * 4;
-  const long wgs = (long)q.nslab * q.nchunk, fit = ((1L << 32) - 1) / ((long)pl.threads * wgs) / 8 * 8;
-  pl.piece = N < fit ? N : fit;  // a grid counts its threads in 32 bits
-  if (pl.piece < 1) pl.piece = 1;
-  return wgs * 8 * pl.threads < (1L << 32);
+  // a grid counts its threads in 32 bits: the sweeps', and the joins' workgroup of 256 per (sample, group)
+  const long wgs = (long)q.nslab * q.nchunk, sweep = wgs * pl.threads, join = pl.split ? (long)G * 256 : 0;
+  const long each = sweep > join ? sweep : join, fit = ((1L << 32) - 1) / each / 8 * 8;
+  pl.piece = N < fit ? N : fit;
+  return fit > 0;
 }
 
 inline bool valid(long N, long P, int C, int G, int vec, int dtype, int per_client) {
   if (N < 1 || P < 1 || C < 1 || G < 1 || C % G || per_client < 1 || N % per_client) return false;
   if (dtype < 0 || dtype > 2 || (vec != 1 && vec != 4) || C % vec) return false;
-  // grids and in-kernel counters are 32 bits, offsets 64
-  return N < (1L << 24) && P < (1L << 30) && (double)N * P * C < 9e15;
+  // grids and in-kernel counters are 32 bits, offsets 64; gn_affine_kernel's grid has C / 8 workgroups of 1024 per client
+  return C <= (1 << 24) && N < (1L << 24) && P < (1L << 30) && (double)N * P * C < 9e15;
 }
 
 }  // namespace groupnorm

@@ -1,6 +1,7 @@
 """Group norm with activation, client-keyed dropout without a stored mask, rotary positions with several axes: the public
 functions against their definitions in 64 bits (CPU and GPU), gradients, refusals, layouts, streams and captured graphs."""
 import math
+import os
 
 import pytest
 import torch
@@ -622,3 +623,30 @@ def test_layers_under_functorch_transforms_use_the_oracle(dev):
     wl = w.clone().requires_grad_(True)
     ops.group_norm(x.reshape(12, 8, 2, 2), 2, wl, act="silu").square().sum().backward()
     torch.testing.assert_close(got, wl.grad, rtol=1e-4, atol=1e-4)
+
+
+@pytest.mark.parametrize("N,P,C,G", [(12693514, 109, 387, 43), (4780147, 238, 327, 109), (1 << 19, 256, 2048, 64),
+                                     (48, 12544, 64, 8)])
+def test_group_norm_plan_counts_every_grid(N, P, C, G):
+    """A launch's threads are counted in 32 bits, and the kernels that join chunks have 256 per (sample, group): read off the
+    plan's workspace, which holds one entry of 8 bytes per sample of a piece, chunk and group."""
+    import ctypes
+
+    from blades_amd.ops import build
+
+    if not os.path.exists(build.HIP_LIB):
+        pytest.skip("kernels are not built")
+    lib = ctypes.CDLL(build.HIP_LIB)
+    lib.blades_group_norm_plan_size.restype = ctypes.c_long
+    buf, ws = ctypes.create_string_buffer(lib.blades_group_norm_plan_size()), (ctypes.c_long * 2)()
+    L, I = ctypes.c_long, ctypes.c_int
+
+    def plan(n, p, c, g):
+        return lib.blades_group_norm_plan(buf, L(n), L(p), I(c), I(g), ctypes.c_float(1e-5), I(0), I(n), L(0), L(0), I(1),
+                                          I(1 if c % 4 else 4), ws)
+
+    assert plan(N, P, C, G) == 0
+    # the backward pass's is N x chunks x C entries and at most N x G for the means
+    chunks = max(1, -(-ws[1] // (N * C * 8)) - 1)
+    assert ws[0] // (8 * chunks) * 256 < 1 << 32
+    assert plan(1, 1, (1 << 24) + 4, 1 << 22) != 0 and plan(1 << 24, 1, 4, 1) != 0
