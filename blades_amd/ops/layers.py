@@ -39,9 +39,12 @@ def _nodes():
     return _loaded
 
 
-def _own_kernel(name: str, t: torch.Tensor) -> bool:
+def _own_kernel(name: str, t: torch.Tensor, *others) -> bool:
     if not t.is_cuda or _ops._FORCE_REFERENCE or _wrapped(t):
         return False
+    for o in others:
+        if o is not None and _wrapped(o):
+            return False
     if t.dtype not in _DTYPES:
         raise ValueError(f"{name}: CUDA tensors must be fp32, bf16 or fp16, got {t.dtype}")
     return True
@@ -77,7 +80,7 @@ def group_norm(x, groups: int, weight=None, bias=None, eps: float = 1e-5, act: s
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
         raise ValueError(f"group_norm: residual must match x ({x.dtype} {tuple(x.shape)}), got {residual.dtype} "
                          f"{tuple(residual.shape)} on {residual.device}")
-    if not _own_kernel("group_norm", x) or x.numel() == 0:
+    if not _own_kernel("group_norm", x, weight, bias, residual) or x.numel() == 0:
         return ref.group_norm(x, groups, weight, bias, eps, act, residual)
     return _nodes().group_norm(x, groups, weight, bias, eps, _ACTS[act], residual)
 
@@ -110,7 +113,7 @@ def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "e
         raise ValueError(f"client_dropout: {tuple(x.shape)} does not divide among {K} clients (layout {layout})")
     if x.numel() == 0:
         return x.clone()
-    if not _own_kernel("client_dropout", x):
+    if not _own_kernel("client_dropout", x, uids, None if by_value else tag):
         return ref.client_dropout(x, uids, seed, tag, layer, p, kind, layout, scale)
     if uids.dim() == 0 or not uids.is_contiguous():
         uids = uids.reshape(-1).contiguous()
@@ -154,6 +157,6 @@ def rope_axes(x, pos, axes, base: float = 10000.0, slots=None):
             len(shape) == 3 and shape[0] != x.shape[0]) or pos.device != x.device or pos.requires_grad:
         raise ValueError(f"rope_axes: pos must be int64 or fp32 [{x.shape[1]}, {len(axes)}] or [{x.shape[0]}, {x.shape[1]}, "
                          f"{len(axes)}] on {x.device} without a gradient, got {pos.dtype} {tuple(shape)} on {pos.device}")
-    if not _own_kernel("rope_axes", x):
+    if not _own_kernel("rope_axes", x, pos):
         return ref.rope_axes(x, pos, axes, base, slots)
     return _nodes().rope_axes(x, pos, axes, base, slots)

@@ -619,7 +619,9 @@ def test_layers_under_functorch_transforms_use_the_oracle(dev):
     def loss(w1, x1):
         return ops.group_norm(x1, 2, w1, act="silu").square().sum()
 
+    g0 = grad(lambda w1: loss(w1, x[0]))(w[0])  # only the weight is wrapped
     got = vmap(grad(loss))(w, x)
+    torch.testing.assert_close(got[0], g0, rtol=1e-4, atol=1e-4)
     wl = w.clone().requires_grad_(True)
     ops.group_norm(x.reshape(12, 8, 2, 2), 2, wl, act="silu").square().sum().backward()
     torch.testing.assert_close(got, wl.grad, rtol=1e-4, atol=1e-4)
