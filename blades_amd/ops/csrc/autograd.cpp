@@ -213,7 +213,9 @@ Tensor drop(const Tensor& t, const Tensor& uids, const Tensor& tag, long tag_val
   }
   Tensor y = at::empty_like(x);
   const int rc = lib.dropout(ptr(x), ptr(y), ptr<long>(uids), ptr<long>(tag), tag_value, &p, stream_of(x));
-  if (rc != 0) throw py::value_error("client_dropout: rejected: a client's share of a layer has at most 1.7e10 elements");
+  if (rc != 0)
+    throw py::value_error("client_dropout: rejected: a client's share of a layer has at most 1.7e10 elements (and at most 2^30 "
+                          "samples, channels and pixels where draws are shared or maps are channels last)");
   return y;
 }
 

@@ -165,8 +165,9 @@ __global__ __launch_bounds__(TPB) void drop_group_kernel(Key key, Rows q, const 
   }
 }
 
-// The same for rows of more channels than a workgroup keeps: every vector's thread makes its own draws.  Memory is walked by vectors of VEC channels (LAST: [sample][pixel][client if
-// inner][C]) or of one channel's pixels (else: [sample][C][pixel]); index arithmetic in I bits.
+// The same for rows of more channels than a workgroup keeps: every vector's thread makes its own draws.  Memory is walked by
+// vectors of VEC channels (LAST: [sample][pixel][client if inner][C]) or of one channel's pixels (else: [sample][C][pixel]);
+// index arithmetic in I bits.
 template <typename T, int VEC, bool LAST, typename I>
 __global__ __launch_bounds__(TPB) void drop_wide_kernel(Key key, const T* __restrict__ x, T* __restrict__ y, int Kc, I B, I C,
                                                          I HW, int inner, int kind, I total) {
@@ -377,9 +378,13 @@ struct DropPlan {
 // tag null: tag_value.
 BLADES_API int blades_client_dropout(const void* x, void* y, const long* uids, const long* tag, long tag_value,
                                      const DropPlan* p, hipStream_t st) {
-  if (p->Kc < 1 || p->B < 1 || p->C < 1 || p->HW < 1 || p->kind < 0 || p->kind > 2 || p->dtype < 0 || p->dtype > 2 || p->least >> 24) return 1;
+  if (p->Kc < 1 || p->B < 1 || p->C < 1 || p->HW < 1 || p->kind < 0 || p->kind > 2 || p->dtype < 0 || p->dtype > 2 ||
+      p->least >> 24)
+    return 1;
   if ((double)p->B * p->C * p->HW > 1.7e10) return 1;  // draws of four are counted in 32 bits
-  if (p->C > (1 << 30) || p->HW > (1 << 30) || p->B > (1 << 30)) return 1;
+  // the kernels that share draws or walk tiles count samples, channels and pixels in 32 bits; drop_elem_kernel in 64
+  const bool tiled = p->kind != 0 || (p->last && p->HW > 1);
+  if (tiled && (p->C > (1 << 30) || p->HW > (1 << 30) || p->B > (1 << 30))) return 2;
   const Key key{uids, tag, tag_value, p->c3, (uint32_t)p->seed, (uint32_t)(p->seed >> 32), p->least << 8, p->scale};
   const int vec = (((uintptr_t)x | (uintptr_t)y) & 15) == 0;  // 16-byte accesses (the lengths permitting)
 #define DROP(T) return dropout_t<T>(key, x, y, p->Kc, p->B, p->C, p->HW, p->kind, p->inner, p->last, vec, st)

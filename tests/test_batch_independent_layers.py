@@ -627,6 +627,36 @@ def test_layers_under_functorch_transforms_use_the_oracle(dev):
     torch.testing.assert_close(got, wl.grad, rtol=1e-4, atol=1e-4)
 
 
+@pytest.mark.gpu
+def test_layers_past_32_bit_offsets(dev):
+    """Tensors of more than 2^32 bytes and 2^31 elements: the last samples are right."""
+    R = (1 << 31) // (64 * 384) + 64
+    x = torch.ones(R, 64, 3, 2, 64, device=dev, dtype=torch.bfloat16)
+    x[-2:] = torch.randn(2, 64, 3, 2, 64, device=dev).to(torch.bfloat16)
+    pos = torch.stack([torch.arange(64, device=dev) // 8, torch.arange(64, device=dev) % 8], -1)
+    y = ops.rope_axes(x, pos, (32, 32), slots=2)
+    rope_near(y[-2:], x[-2:], rope64(x[-2:], pos, (32, 32), 10000.0, 2), torch.bfloat16)
+    del y
+    v = x.view(-1)[: ((1 << 31) + 4096 * 8) // 64 * 64]
+    uids = torch.tensor([3, 8], device=dev)
+    a = v[: v.numel() // 2 * 2].view(2, -1)
+    y = ops.client_dropout(a, uids, 9, 4, 1, 0.25)
+    n = a.shape[1]
+    m = ref.client_dropout_mult(uids[1:].cpu(), 4, 9, 4, 1, 0.25)  # the start of the second client's share
+    assert torch.equal((y[1, :4] != 0).cpu(), (a[1, :4].cpu() * m[0].to(torch.bfloat16)) != 0)
+    tail = ref._philox4x32(*(torch.tensor([t]) for t in ((n - 4) >> 2, 8, 4, 2 + 256)), 9, 0)
+    keep = torch.tensor([(int(w) >> 8) * 2.0 ** -24 >= 0.25 for w in tail])
+    want = torch.where(keep, a[1, -4:].cpu().double() / 0.75, torch.zeros(4, dtype=torch.float64))
+    torch.testing.assert_close(y[1, -4:].cpu().double(), want, rtol=half_step(torch.bfloat16) + 4 * U32, atol=0)
+    del y, a, v
+    N = (1 << 31) // (64 * 1024) + 3
+    x = x.view(-1)[: N * 65536].view(N, 32, 32, 64).permute(0, 3, 1, 2)
+    x[-2:] = torch.randn(2, 64, 32, 32, device=dev).to(torch.bfloat16)
+    y = ops.group_norm(x, 32, act="silu")
+    want = gn64(x[-2:], 32, None, None, 1e-5, "silu", None, x[-2:])
+    assert bool(((y[-2:].double() - want["y"]).abs() <= 4 * 512 * U32 * 8 + half_step(torch.bfloat16) * want["y"].abs()).all())
+
+
 @pytest.mark.parametrize("N,P,C,G", [(12693514, 109, 387, 43), (4780147, 238, 327, 109), (1 << 19, 256, 2048, 64),
                                      (48, 12544, 64, 8)])
 def test_group_norm_plan_counts_every_grid(N, P, C, G):
