@@ -1903,7 +1903,7 @@ def group_norm_supported(x: torch.Tensor, groups: int) -> bool:
         return False
     N, C = x.shape[0], x.shape[1]
     return C % groups == 0 and _gn_plan(N, x.numel() // (N * C), C, groups, 1e-5, 0, N, 0, 0, _DT_CODE[x.dtype],
-                                        1).ws is not None
+                                        1 if C % 4 else 4).ws is not None
 
 
 def _gn_check(name, x, groups, clients, weight, bias, *others):

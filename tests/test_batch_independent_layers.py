@@ -627,6 +627,94 @@ def test_layers_under_functorch_transforms_use_the_oracle(dev):
     torch.testing.assert_close(got, wl.grad, rtol=1e-4, atol=1e-4)
 
 
+def layer_calls(dev):
+    x = last(torch.randn(6, 8, 4, 4)).to(dev)
+    uids, tag = torch.arange(3, device=dev), torch.ones(1, dtype=torch.int64, device=dev)
+    pos = torch.arange(8, device=dev).unsqueeze(1)
+    return x, [lambda t: ops.group_norm(t, 2, act="gelu"), lambda t: ops.client_dropout(t, uids, 1, tag, 0, 0.5),
+               lambda t: ops.client_dropout(t, uids, 1, 7, 0, 0.5), lambda t: ops.rope_axes(t, pos, (4,))]
+
+
+@pytest.mark.gpu
+def test_layers_autograd_contract(dev):
+    """A second backward pass needs retain_graph, a second differentiation raises, a changed input raises, and gradients
+    reach a graph in front of the layer."""
+    x, calls = layer_calls(dev)
+    for f in calls:
+        a = x.clone(memory_format=torch.preserve_format).requires_grad_(True)
+        y = f(a)
+        gy = torch.randn_like(y)
+        g1 = torch.autograd.grad(y, a, gy, retain_graph=True)[0]
+        assert torch.equal(torch.autograd.grad(y, a, gy)[0], g1)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(y, a, gy)
+        (g2,) = torch.autograd.grad(f(a), a, gy, create_graph=True)
+        assert torch.equal(g2, g1)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g2.sum(), a)
+        torch.testing.assert_close(torch.autograd.grad(f(a * 1.0), a, gy)[0], g1)
+        with torch.no_grad():
+            z = f(a)
+        assert not z.requires_grad and torch.equal(z, y)
+        with torch.inference_mode():
+            assert torch.equal(f(x), y)
+    a = x.clone(memory_format=torch.preserve_format).requires_grad_(True)
+    b = a * 1.0
+    y = ops.group_norm(b, 2)
+    with torch.no_grad():
+        b.add_(1)
+    with pytest.raises(RuntimeError):
+        y.sum().backward()
+    # the same tensor as input and residual, and as a layer's only leaf twice
+    a = x.clone(memory_format=torch.preserve_format).requires_grad_(True)
+    ops.group_norm(a, 2, act="silu", residual=a).sum().backward()
+    c = x.double().cpu().requires_grad_(True)
+    ops.group_norm(c, 2, act="silu", residual=c).sum().backward()
+    assert float((a.grad.cpu().double() - c.grad).abs().max()) <= 2 * 512 * U32 * 40
+
+
+@pytest.mark.gpu
+def test_layers_from_two_threads_and_streams(dev):
+    """Calls from two threads on two streams at once give what one gives alone."""
+    import threading
+
+    x, calls = layer_calls(dev)
+    x = x.repeat(50, 1, 1, 1).contiguous(memory_format=torch.channels_last)
+
+    def work(out):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.default_stream())
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                a = x.detach().requires_grad_(True)
+                res = []
+                for f in calls[:3]:
+                    y = f(a)
+                    res += [y.detach(), torch.autograd.grad(y, a, x)[0]]
+                out[:] = res
+        s.synchronize()
+
+    torch.cuda.synchronize()
+    want, outs = [], [[], []]
+    work(want)
+    threads = [threading.Thread(target=work, args=(o,)) for o in outs]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    for o in outs:
+        assert len(o) == len(want) and all(torch.equal(p, q) for p, q in zip(o, want))
+
+
+@pytest.mark.gpu
+def test_layers_many_small_samples(dev):
+    """More samples than a grid of workgroups holds at once, one pixel each; offsets stay right to the last row."""
+    N = (1 << 22) + 5
+    x = torch.randn(N, 8, device=dev)
+    y = ops.group_norm(x, 2, act="relu")
+    for rows in (slice(0, 3), slice(N - 3, N), slice((1 << 21) - 2, (1 << 21) + 2)):
+        want = gn64(x[rows], 2, None, None, 1e-5, "relu", None, x[rows])["y"]
+        assert float((y[rows].double() - want).abs().max()) <= 2 * 512 * U32 * 4
+
+
 @pytest.mark.gpu
 def test_layers_past_32_bit_offsets(dev):
     """Tensors of more than 2^32 bytes and 2^31 elements: the last samples are right."""
