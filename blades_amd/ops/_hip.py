@@ -1879,16 +1879,15 @@ def _gn_plan(N, P, C, G, eps, act, per_client, gstride, bstride, dt, vec):
     return plan
 
 
-def group_norm_plan(x, G, eps, act, clients, weight, bias, *others, vec=0):
+def group_norm_plan(x, G, eps, act, clients, weight, bias, *others):
     """Plan for channels-last ``x``: four channels per access where their count and every address allow them."""
     shape = x.shape
     N, C = shape[0], shape[1]
-    if not vec:
-        a = x.data_ptr()
-        for t in others:
-            if t is not None:
-                a |= t.data_ptr()
-        vec = 1 if C % 4 or a % 16 else 4
+    a = x.data_ptr()
+    for t in others:
+        if t is not None:
+            a |= t.data_ptr()
+    vec = 1 if C % 4 or a % 16 else 4
     plan = _gn_plan(N, x.numel() // (N * C), C, G, eps, ACT_CODE[act], N // clients,
                     0 if weight is None or weight.dim() == 1 else weight.stride(0),
                     0 if bias is None or bias.dim() == 1 else bias.stride(0), _DT_CODE[x.dtype], vec)
@@ -1971,11 +1970,9 @@ def group_norm_backward(x, gy, groups: int, weight, bias, stats, plan, act: str 
             raise ValueError("group_norm_backward: the gate does not match x")
     x, gy = to_channels_last(x), to_channels_last(gy)
     residual = None if residual is None or gate is not None else to_channels_last(residual)
-    if plan.vec > 1 and (x.data_ptr() | gy.data_ptr() | (0 if residual is None else residual.data_ptr())) % 16:
-        if gate is None:
-            plan = group_norm_plan(x, groups, 0.0, act, clients, weight, bias, vec=1)
-        else:  # the gate's vectors decide
-            x, gy = (t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.preserve_format) for t in (x, gy))
+    if plan.vec > 1:  # the forward pass's accesses, and its gate's
+        x, gy, residual = (t if t is None or t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.preserve_format)
+                           for t in (x, gy, residual))
     dx = _like_channels_last(x) if want_dx else None
     dres = _like_channels_last(x) if want_dres else None
     ws = _empty(plan.ws[1], dtype=torch.uint8, device=x.device)

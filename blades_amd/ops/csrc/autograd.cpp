@@ -43,6 +43,14 @@ int dtype_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? 0 : t.sca
 
 template <typename T = void> T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
 
+// Saved tensors can pass through hooks (moved to the host and back, say): the kernels rely on these.
+void check_saved(const char* name, bool ok) {
+  TORCH_CHECK(ok, name, ": a saved tensor came back with another shape, type or device");
+}
+bool like(const Tensor& t, const Tensor& r) {
+  return !t.defined() || (t.sizes() == r.sizes() && t.scalar_type() == r.scalar_type() && t.device() == r.device());
+}
+
 bool needs_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
 bool channels_last(const Tensor& t) {
@@ -73,19 +81,25 @@ variable_list first_order(variable_list&& grads) {
 // ---------------------------------------------------------------------------------------------------------------
 struct GroupNorm {
   std::vector<char> plan;
-  long ws[2];
+  long ws[2], strides[2];  // (of the weight and the bias, client to client)
   int vec, groups, act;
   long clients;
   float eps;
 
+  static long stride(const Tensor& t) { return t.defined() && t.dim() == 2 ? t.stride(0) : 0; }
+  bool affine_fits(const Tensor& t, const Tensor& x, long C) const {
+    return !t.defined() || (t.scalar_type() == at::kFloat && t.device() == x.device() && t.dim() > 0 && t.size(-1) == C &&
+                            (t.dim() == 1 || (t.dim() == 2 && t.size(0) == clients)));
+  }
+
   void make(const Tensor& x, const Tensor& w, const Tensor& b, int v) {
     const long N = x.size(0), C = x.size(1), P = x.numel() / (N * C);
     plan.resize(lib.gn_plan_size());
-    auto stride = [](const Tensor& t) { return t.defined() && t.dim() == 2 ? t.stride(0) : 0; };
+    strides[0] = stride(w); strides[1] = stride(b);
     auto fill = [&](int channels) {
       vec = channels;
-      return lib.gn_plan(plan.data(), N, P, (int)C, groups, eps, act, (int)(N / clients), stride(w), stride(b), dtype_of(x), vec,
-                         ws);
+      return lib.gn_plan(plan.data(), N, P, (int)C, groups, eps, act, (int)(N / clients), strides[0], strides[1], dtype_of(x),
+                         vec, ws);
     };
     int rc = fill(v);
     if (rc == 2 && v > 1) rc = fill(1);  // wide groups of an odd number of channels
@@ -99,6 +113,12 @@ struct GroupNorm {
 bool aligned(const Tensor& a, const Tensor& b, const Tensor& c) {
   return ((reinterpret_cast<uintptr_t>(ptr(a)) | reinterpret_cast<uintptr_t>(ptr(b)) | reinterpret_cast<uintptr_t>(ptr(c))) &
           15) == 0;
+}
+
+Tensor affine(const Tensor& t) {
+  if (!t.defined()) return t;
+  Tensor f = t.scalar_type() == at::kFloat ? t : t.to(at::kFloat);
+  return f.stride(-1) == 1 ? f : f.contiguous();
 }
 
 struct GroupNormBackward : Node {
@@ -122,19 +142,27 @@ variable_list GroupNormBackward::apply(variable_list&& grads) {
              nb = has_b && task_should_compute_output(2), nr = has_res && task_should_compute_output(3);
   {
     at::NoGradGuard no_grad;
-    Tensor x_ = x.unpack(shared_from_this()), w_ = w.unpack(shared_from_this()), b_ = b.unpack(shared_from_this());
-    Tensor st = stats.unpack(shared_from_this()), r_ = res.unpack(shared_from_this()), gt = gate.unpack(shared_from_this());
-    const c10::DeviceGuard guard(x_.device());
-    Tensor g_ = to_channels_last(gy);
+    const auto self = shared_from_this();
+    Tensor x_ = x.unpack(self), r_ = res.unpack(self), w_ = w.unpack(self), b_ = b.unpack(self);
+    Tensor st = stats.unpack(self), gt = gate.unpack(self);
     std::shared_ptr<GroupNorm> p = g;
-    if (p->vec > 1 && !aligned(x_, g_, r_)) {
-      if (gt.defined()) {  // the gate's vectors decide
-        g_ = g_.clone(at::MemoryFormat::Preserve);
-      } else {
-        p = std::make_shared<GroupNorm>(*g);
-        p->make(x_, w_, b_, 1);
-      }
+    const int64_t C = gy.size(1);
+    check_saved("group_norm", like(x_, gy) && like(r_, gy) && p->affine_fits(w_, gy, C) && p->affine_fits(b_, gy, C) &&
+                st.scalar_type() == at::kFloat && st.device() == gy.device() && st.numel() == 2 * gy.size(0) * p->groups &&
+                (!gt.defined() || (gt.scalar_type() == at::kByte && gt.device() == gy.device() &&
+                                   gt.numel() * p->vec == gy.numel())));
+    Tensor g_ = to_channels_last(gy);
+    x_ = to_channels_last(x_); r_ = to_channels_last(r_);
+    w_ = affine(w_); b_ = affine(b_); st = st.contiguous();
+    if (gt.defined()) gt = gt.contiguous();
+    const c10::DeviceGuard guard(x_.device());
+    if (GroupNorm::stride(w_) != p->strides[0] || GroupNorm::stride(b_) != p->strides[1]) {
+      p = std::make_shared<GroupNorm>(*g);
+      p->make(x_, w_, b_, g->vec);
     }
+    if (p->vec > 1)
+      for (Tensor* t : {&x_, &g_, &r_})
+        if (!aligned(*t, Tensor(), Tensor())) *t = t->clone(at::MemoryFormat::Preserve);
     const auto f32 = x_.options().dtype(at::kFloat);
     const bool own_dres = nr && p->act != 0;
     if (nx) out[0] = like_channels_last(x_);
@@ -149,12 +177,6 @@ variable_list GroupNormBackward::apply(variable_list&& grads) {
     if (nb && b_type != at::kFloat) out[2] = out[2].to(b_type);
   }
   return first_order(std::move(out));
-}
-
-Tensor affine(const Tensor& t) {
-  if (!t.defined()) return t;
-  Tensor f = t.scalar_type() == at::kFloat ? t : t.to(at::kFloat);
-  return f.stride(-1) == 1 ? f : f.contiguous();
 }
 
 Tensor group_norm(const Tensor& x, int64_t groups, const MaybeTensor& weight, const MaybeTensor& bias, double eps, int64_t act,
@@ -204,6 +226,9 @@ struct DropPlan {  // as in dropout.hip
 };
 
 Tensor drop(const Tensor& t, const Tensor& uids, const Tensor& tag, long tag_value, DropPlan p) {
+  check_saved("client_dropout", uids.numel() == p.Kc && uids.scalar_type() == at::kLong && uids.device() == t.device() &&
+              uids.is_contiguous() && (!tag.defined() || (tag.numel() == 1 && tag.scalar_type() == at::kLong &&
+              tag.device() == t.device())));
   const c10::DeviceGuard guard(t.device());
   Tensor x = t;
   p.last = 0;
@@ -300,6 +325,9 @@ std::shared_ptr<std::vector<char>> rope_plan(const Tensor& x, const Tensor& pos,
 Tensor turn(const Tensor& t, const Tensor& pos, const Rope& r, int inverse) {
   const c10::DeviceGuard guard(t.device());
   if (t.numel() == 0) return at::empty(t.sizes(), t.options());
+  check_saved("rope_axes", (pos.scalar_type() == at::kFloat || pos.scalar_type() == at::kLong) && pos.device() == t.device() &&
+              (pos.dim() == 2 || (pos.dim() == 3 && pos.size(0) == t.size(0))) && pos.size(-2) == t.size(1) &&
+              pos.size(-1) == (int64_t)r.axes.size());
   Tensor x = t.stride(-1) == 1 ? t : t.contiguous();
   const Tensor p = pos.contiguous();
   const int w = x.scalar_type() == at::kFloat ? 4 : 8;

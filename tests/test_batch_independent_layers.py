@@ -674,6 +674,73 @@ def test_layers_autograd_contract(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("how", ["contiguous", "host", "shifted"])
+def test_saved_tensors_that_move(dev, how):
+    """Saved tensors may come back from hooks with other strides, from the host, or at other addresses."""
+    def unpack(t):
+        if how == "host":
+            return t.to(dev)
+        if how == "contiguous" or t.dim() == 0:
+            return t
+        buf = torch.empty(t.numel() + 1, dtype=t.dtype, device=dev)[1:].view(t.shape)  # off by one element
+        return buf.copy_(t)
+
+    def pack(t):
+        return t.cpu() if how == "host" else t.contiguous().clone()
+
+    K, C = 3, 16
+    rows = torch.randn(K, 5 * C, device=dev)  # per-client affine vectors inside longer rows
+    x = last(torch.randn(6, C, 5, 5, device=dev))
+    r = last(torch.randn(6, C, 5, 5, device=dev))
+    gy = torch.randn(6, C, 5, 5, device=dev)
+    uids, tag = torch.arange(3, device=dev), torch.ones(1, dtype=torch.int64, device=dev)
+    pos = torch.arange(C, device=dev).unsqueeze(1)
+
+    def grads():
+        out = []
+        for act in ("none", "relu", "gelu"):
+            leaves = [t.detach().requires_grad_(True) for t in (x, rows[:, C:2 * C], rows[:, 3 * C:4 * C], r)]
+            a, w, b, s = leaves
+            assert w.stride(0) == 5 * C
+            out += torch.autograd.grad(ops.group_norm(a, 4, w, b, act=act, residual=s), leaves, gy)
+        shared = rows[0, :C].detach().requires_grad_(True)
+        out += torch.autograd.grad(ops.group_norm(x, 4, shared.expand(K, C), None, act="silu"), shared, gy)
+        a = x.detach().requires_grad_(True)
+        out += torch.autograd.grad(ops.client_dropout(a, uids, 1, tag, 0, 0.5), a, gy)
+        a = torch.empty_like(gy[..., :4]).copy_(gy[..., :4]).requires_grad_(True)
+        return out + list(torch.autograd.grad(ops.rope_axes(a, pos, (4,)), a, gy[..., :4]))
+
+    want = grads()
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        got = grads()
+    for g, w in zip(got, want):
+        assert torch.equal(g, w)
+
+
+@pytest.mark.gpu
+def test_saved_tensors_that_change_are_refused(dev):
+    x, calls = layer_calls(dev)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.reshape(-1)[:1].clone()):
+        for f in calls:
+            a = x.clone(memory_format=torch.preserve_format).requires_grad_(True)
+            y = f(a)
+            with pytest.raises(RuntimeError, match="saved tensor"):
+                y.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_group_norm_gradient_at_any_address(dev, act):
+    """Groups of more than 1024 channels need accesses of four: a gradient at an odd address is brought in line."""
+    x = last(torch.randn(2, 2048, 3, device=dev)).requires_grad_(True)
+    gy = torch.randn(2 * 3 * 2048 + 1, device=dev)[1:].view(2, 3, 2048).movedim(-1, 1)
+    y = ops.group_norm(x, 1, act=act)
+    (g1,) = torch.autograd.grad(y, x, gy, retain_graph=True)
+    (g2,) = torch.autograd.grad(y, x, last(gy.clone()))
+    assert gy.data_ptr() % 16 and torch.equal(g1, g2)
+
+
+@pytest.mark.gpu
 def test_layers_from_two_threads_and_streams(dev):
     """Calls from two threads on two streams at once give what one gives alone."""
     import threading
