@@ -3,13 +3,13 @@
 * ``libblades_host.so``  — g++,  ``csrc/host.cpp``  (CPU; clustering, partitioner)
 * ``libblades_hip.so``   — hipcc ``--offload-arch=gfx950``, every ``csrc/*.hip``
 
-Both expose a plain C ABI and are loaded with ctypes, so neither needs the
-PyTorch headers: a full rebuild is seconds, and hipcc cross-compiles gfx950
-code objects on a machine without a GPU.
-
 * ``_autograd.so``       — g++, ``csrc/autograd.cpp`` (no device code): the autograd
   nodes of ``ops/layers.py``, the one file that includes PyTorch's headers; it calls
   ``libblades_hip.so`` through addresses
+
+The two libraries expose a plain C ABI and are loaded with ctypes, so neither needs
+the PyTorch headers: a full rebuild is seconds, and hipcc cross-compiles gfx950
+code objects on a machine without a GPU.
 """
 import os
 import re

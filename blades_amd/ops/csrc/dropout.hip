@@ -6,6 +6,10 @@
 // the layout in memory, so the mask depends on (seed, client, tag, layer) alone and equals client_dropout_mult's.
 // `tag` may live in device memory: a captured HIP graph then replays with the current round's.
 //
+// Bound by the generator (element draws: 18 64-bit products and 34 exclusive ors per draw of four) and memory alike: 32 x 64 x
+// 64 x 128 fp32 22 us (134 MB, 6.0 TB/s; the bytes alone 17 at the cache's 8), and by memory where a draw is shared: 3840 x 64
+// x 6 x 6 bf16 by channel 9.7 (35 MB).  Outputs are stored through the caches: what follows reads them at once.
+//
 // Multiplication, not selection, as the stored multipliers had it: 0 * inf stays NaN.
 #include "common.h"
 

@@ -13,7 +13,7 @@
 // cancellation for offset activations), then the result, all from registers.  Lane l of a pixel row owns VEC channels
 // (four, or one where the channel count or an address does not allow it), so a thread keeps its channels for the whole sweep.
 // A sample too large for a workgroup's registers is
-// cut into pixel chunks: a first sweep leaves (mean, M2) or (A, B) of each, a small kernel joins them in chunk order, and a
+// cut into pixel chunks: a first sweep leaves (mean, M2) or (A, B) of each, small kernels join them in chunk order, and a
 // second sweep applies, from the last sample to the first: what the first sweep read last is still in the 256 MB cache
 // (walking the batch in pieces that fit it as a whole costs more in launches than it saves: 48 x 64 x 112 x 112 fp32
 // forward + backward 380 us in pieces of 96 MB, 319 in 180 MB, 292 at once).  All sums are fp32 in a fixed order (double

@@ -1,7 +1,7 @@
 """Differentiable layers whose result for one sample does not depend on who shares its batch.
 
 * ``group_norm``     — group normalisation + residual add + activation, channels last, one affine pair for everybody or
-  one per client (ops/csrc/groupnorm.hip); the normalisation of federated models whose clients' data differ, and of
+  one per client (ops/csrc/groupnorm_{fwd,bwd}.hip); the normalisation of federated models whose clients' data differ, and of
   differentially private ones, which a batch statistic would leak
 * ``client_dropout`` — dropout from a counter-based generator keyed by the client, drawn again in the backward pass
   instead of stored (ops/csrc/dropout.hip)
@@ -10,7 +10,8 @@
 
 CUDA tensors run the hand-written kernels (fp32, bf16 or fp16; anything else raises), CPU tensors and tensors wrapped by
 ``torch.func`` transforms the oracles of ``reference.py``.  Arguments are checked alike on both.  The gradients are
-first-order: differentiating them again raises.  The autograd nodes are C++ (csrc/autograd.cpp): both passes run without
+first-order: differentiating them again raises.  As with any operator, a backward pass is captured into a graph with no
+eager graph of the same leaves alive: what that one left on the leaves belongs to its stream.  The autograd nodes are C++ (csrc/autograd.cpp): both passes run without
 the interpreter.
 """
 import functools

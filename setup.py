@@ -1,9 +1,9 @@
 """Packaging for blades_amd.
 
 ``pip install -e .`` (or ``python setup.py build_native``) compiles the native libraries in-tree —
-``libblades_hip.so`` (hipcc, gfx950), ``libblades_host.so`` (g++) and the ``blades_launch`` process launcher — with
-the same builder the tests and ``__graft_entry__.build()`` use (``blades_amd/ops/build.py``: plain C ABI, ctypes, no
-PyTorch headers), and ships them as package data.  The ``blades`` / ``fllib`` packages are import shims for code
+``libblades_hip.so`` (hipcc, gfx950), ``libblades_host.so`` (g++), ``_autograd.so`` (g++) and the ``blades_launch`` process launcher — with
+the same builder the tests and ``__graft_entry__.build()`` use (``blades_amd/ops/build.py``: plain C ABI, ctypes;
+PyTorch's headers in ``_autograd.so`` alone), and ships them as package data.  The ``blades`` / ``fllib`` packages are import shims for code
 written against the reference (``from blades.algorithms.fedavg import FedavgConfig``).
 """
 import os
