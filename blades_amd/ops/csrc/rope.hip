@@ -8,10 +8,10 @@
 // others copied (v).  A thread owns 16 bytes of the head dimension of one token: while its first rows are on their way, its two
 // (four) angles are computed, once for all its rows (slots and heads): the turns (position times frequency, reduced to an
 // eighth) in 64 bits so that far positions keep theirs, sine and cosine by their Taylor polynomials in 32 bits.
-// Memory-bound: every byte is read and written once.  Measured: 2048 x 64 x 3 x 2 x 64 fp32 74 us (5.4 TB/s), 8 x 3136 x 3 x 6 x
-// 64 bf16 with per-sample positions 23 (5.0; 19 without the angles).  (A workgroup that shares its tokens' angles through LDS and walks
-// memory in order was slower, 95 against 73 us on 2048 x 64 x 3 x 2 x 64 fp32: the index arithmetic of every vector and
-// half the waves cost more than the angles.)
+// Memory-bound: every byte is read and written once.  Measured: 2048 x 64 x 3 x 2 x 64 fp32 74 us (5.4 TB/s), 8 x 3136 x 3 x
+// 6 x 64 bf16 with per-sample positions 23 (5.0; 19 without the angles).  (A workgroup that shares its tokens' angles through
+// LDS and walks memory in order was slower, 95 against 73 us on the first: the index arithmetic of every vector and half the
+// waves cost more than the angles.)
 #include "common.h"
 
 namespace {

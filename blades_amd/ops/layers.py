@@ -11,8 +11,8 @@
 CUDA tensors run the hand-written kernels (fp32, bf16 or fp16; anything else raises), CPU tensors and tensors wrapped by
 ``torch.func`` transforms the oracles of ``reference.py``.  Arguments are checked alike on both.  The gradients are
 first-order: differentiating them again raises.  As with any operator, a backward pass is captured into a graph with no
-eager graph of the same leaves alive: what that one left on the leaves belongs to its stream.  The autograd nodes are C++ (csrc/autograd.cpp): both passes run without
-the interpreter.
+eager graph of the same leaves alive: what that one left on the leaves belongs to its stream.  The autograd nodes are C++
+(csrc/autograd.cpp): both passes run without the interpreter.
 """
 import functools
 import math
@@ -120,8 +120,8 @@ def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "e
         uids = uids.reshape(-1).contiguous()
     least, times = _draw(p)
     code = 0 if kind == "elem" or (kind == "channel" and x.dim() <= 2) else 1 if kind == "channel" else 2
-    return _nodes().client_dropout(x, uids, None if by_value else tag, int(tag) & 0xFFFFFFFF if by_value else 0, int(seed) & (2 ** 64 - 1),
-                                   (2 + 256 * int(layer)) & 0xFFFFFFFF, least, times if scale is None else float(scale), code,
+    return _nodes().client_dropout(x, uids, None if by_value else tag, int(tag) & 0xFFFFFFFF if by_value else 0,
+                                   int(seed) & (2 ** 64 - 1), (2 + 256 * int(layer)) & 0xFFFFFFFF, least, times if scale is None else float(scale), code,
                                    inner)
 
 
