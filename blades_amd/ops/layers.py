@@ -8,8 +8,8 @@
 * ``rope_axes``      — rotary positions with several axes for image and video tokens: no table whose length ties the
   parameters to one image size (ops/csrc/rope.hip)
 
-CUDA tensors run the hand-written kernels (fp32, bf16 or fp16; anything else raises), CPU tensors and tensors wrapped by
-``torch.func`` transforms the oracles of ``reference.py``.  Arguments are checked alike on both.  The gradients are
+CUDA tensors run the hand-written kernels (fp32, bf16 or fp16; anything else raises), CPU tensors, tensors wrapped by
+``torch.func`` transforms and those with a forward-mode tangent the oracles of ``reference.py``.  Arguments are checked alike on both.  The gradients are
 first-order: differentiating them again raises.  As with any operator, a backward pass is captured into a graph with no
 eager graph of the same leaves alive: what that one left on the leaves belongs to its stream.  The autograd nodes are C++
 (csrc/autograd.cpp): both passes run without the interpreter.
@@ -19,6 +19,7 @@ import math
 from ctypes import c_float
 
 import torch
+from torch.autograd import forward_ad
 
 import blades_amd.ops as _ops
 
@@ -33,6 +34,11 @@ _wrapped = torch._C._functorch.is_functorch_wrapped_tensor
 _loaded = None
 
 
+def _tangent(t) -> bool:
+    """Does ``t`` carry a forward-mode tangent?  The nodes of csrc/autograd.cpp know reverse mode alone."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
 def _nodes():
     global _loaded
     if _loaded is None:
@@ -41,10 +47,10 @@ def _nodes():
 
 
 def _own_kernel(name: str, t: torch.Tensor, *others) -> bool:
-    if not t.is_cuda or _ops._FORCE_REFERENCE or _wrapped(t):
+    if not t.is_cuda or _ops._FORCE_REFERENCE or _wrapped(t) or _tangent(t):
         return False
     for o in others:
-        if o is not None and _wrapped(o):
+        if o is not None and (_wrapped(o) or _tangent(o)):
             return False
     if t.dtype not in _DTYPES:
         raise ValueError(f"{name}: CUDA tensors must be fp32, bf16 or fp16, got {t.dtype}")
