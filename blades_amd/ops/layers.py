@@ -9,7 +9,8 @@
   parameters to one image size (ops/csrc/rope.hip)
 
 CUDA tensors run the hand-written kernels (fp32, bf16 or fp16; anything else raises), CPU tensors, tensors wrapped by
-``torch.func`` transforms and those with a forward-mode tangent the oracles of ``reference.py``.  Arguments are checked alike on both.  The gradients are
+``torch.func`` transforms, tensor subclasses that define their operations, those with a forward-mode tangent, and calls that
+are traced or run under a dispatch mode the oracles of ``reference.py``.  Arguments are checked alike on both.  The gradients are
 first-order: differentiating them again raises.  As with any operator, a backward pass is captured into a graph with no
 eager graph of the same leaves alive: what that one left on the leaves belongs to its stream.  The autograd nodes are C++
 (csrc/autograd.cpp): both passes run without the interpreter.
@@ -31,6 +32,7 @@ _P_END = 1.0 - 2.0 ** -25  # rounds to 1 in 32 bits from here
 _POS = (torch.int64, torch.float32)
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _wrapped = torch._C._functorch.is_functorch_wrapped_tensor
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
 _loaded = None
 
 
@@ -46,11 +48,27 @@ def _nodes():
     return _loaded
 
 
+def _recorded() -> bool:
+    """Is somebody listening to the operations (``torch.jit.trace``, ``make_fx``, fake tensors, selective checkpoints)?  Of a
+    kernel launched by address they would see the allocations alone."""
+    return torch._C._is_tracing() or torch._C._len_torch_dispatch_stack() > 0
+
+
+def _wrapper(t) -> bool:
+    """A tensor subclass that defines its operations itself (and may have no memory of its own)."""
+    return type(t) not in _PLAIN and torch._C._dispatch_keys(t).has(torch._C.DispatchKey.Python)
+
+
+def _elementary(t) -> bool:
+    """Must ``t`` go through operations that PyTorch sees?"""
+    return _wrapped(t) or _wrapper(t) or _tangent(t)
+
+
 def _own_kernel(name: str, t: torch.Tensor, *others) -> bool:
-    if not t.is_cuda or _ops._FORCE_REFERENCE or _wrapped(t) or _tangent(t):
+    if not t.is_cuda or _ops._FORCE_REFERENCE or _recorded() or _elementary(t):
         return False
     for o in others:
-        if o is not None and (_wrapped(o) or _tangent(o)):
+        if o is not None and _elementary(o):
             return False
     if t.dtype not in _DTYPES:
         raise ValueError(f"{name}: CUDA tensors must be fp32, bf16 or fp16, got {t.dtype}")

@@ -437,7 +437,7 @@ def group_norm(x, groups: int, weight=None, bias=None, eps: float = 1e-5, act: s
 
     def per_sample(t):
         t = t.to(acc)
-        return t.reshape(1, C, *tail) if t.dim() == 1 else t.repeat_interleave(N // t.shape[0], dim=0).reshape(N, C, *tail)
+        return t.reshape(1, C, *tail) if t.dim() == 1 else t.repeat_interleave(int(N // t.shape[0]), dim=0).reshape(N, C, *tail)
 
     if weight is not None:
         z = z * per_sample(weight)
@@ -457,9 +457,11 @@ def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "e
     Kc = uids.numel()
     keep = 1 if kind == "sample" else (2 if kind == "channel" and x.dim() > 2 else x.dim())
     if layout == "major":
-        lead, B, C = [Kc, x.shape[0] // Kc], x.shape[0] // Kc, (x.shape[1] if x.dim() > 1 else 1)
+        B, C = int(x.shape[0] // Kc), int(x.shape[1]) if x.dim() > 1 else 1
+        lead = [Kc, B]
     else:
-        lead, B, C = [x.shape[0], Kc], x.shape[0], x.shape[1] // Kc
+        B, C = int(x.shape[0]), int(x.shape[1] // Kc)
+        lead = [B, Kc]
     value = [1 if i >= keep else (C if i == 1 else int(d)) for i, d in enumerate(x.shape)][1:]  # draws of one sample
     n = B
     for d in value:

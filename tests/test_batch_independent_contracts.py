@@ -75,3 +75,77 @@ def test_engine_dropout_forward_mode(dev):
     with forward_ad.dual_level():
         y = m(forward_ad.make_dual(x, d))
         assert torch.equal(forward_ad.unpack_dual(y).tangent, torch.where(m(x) != 0, 2 * d, 0 * d))
+
+
+class Doubled(torch.Tensor):
+    """A subclass without memory of its own: stands for twice the tensor inside."""
+
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_wrapper_subclass(cls, t.shape, strides=t.stride(), dtype=t.dtype, device=t.device)
+
+    def __init__(self, t):
+        self.t = t
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        def full(a):
+            return a.t * 2 if isinstance(a, Doubled) else a
+
+        return func(*torch.utils._pytree.tree_map(full, args), **torch.utils._pytree.tree_map(full, kwargs or {}))
+
+
+class Tagged(torch.Tensor):
+    """A subclass that leaves the operations alone."""
+
+
+def test_who_must_see_the_operations():
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from blades_amd.ops import layers as mod
+
+    t = torch.zeros(2, 3)
+    assert not mod._elementary(t) and not mod._elementary(torch.nn.Parameter(t)) and not mod._recorded()
+    assert not mod._elementary(t.as_subclass(Tagged)) and mod._elementary(Doubled(t))
+    seen = []
+
+    def probe(a):
+        seen.append(mod._recorded())
+        return a + 1
+
+    torch.jit.trace(probe, (t,), check_trace=False)
+    make_fx(probe)(t)
+    make_fx(probe, tracing_mode="fake")(t)
+    assert len(seen) >= 3 and all(seen) and not mod._recorded()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("how", ["trace", "fx", "fake"])
+@pytest.mark.parametrize("name", LAYERS)
+@pytest.mark.filterwarnings("ignore")
+def test_recorded_calls(dev, name, how):
+    """A recorded layer computes other inputs' results (not the memory its allocations find), and recording works on tensors
+    without memory."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    f, args = layers(dev)[name]
+
+    def g(*a):
+        return f(a)
+
+    rec = torch.jit.trace(g, tuple(args), check_trace=False) if how == "trace" else make_fx(
+        g, tracing_mode="real" if how == "fx" else "fake", _allow_non_fake_inputs=True)(*args)
+    new = [2 * a + 1 for a in args]
+    want, got = f(new), rec(*new)
+    # two fp32 forms of the same values, each within 512 half steps of (1 + |x of a unit spread|) <= 5 times a slope of 1.13
+    assert float((got - want).abs().max()) <= 2 * 512 * U32 * 5 * 1.13 * max(1.0, float(want.abs().max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", LAYERS)
+def test_tensor_subclasses(dev, name):
+    f, args = layers(dev)[name]
+    plain = f([2 * args[0]] + args[1:])
+    assert torch.equal(f([(2 * args[0]).as_subclass(Tagged)] + args[1:]).as_subclass(torch.Tensor), plain)
+    got = f([Doubled(args[0])] + args[1:])
+    assert float((got - plain).abs().max()) <= 2 * 512 * U32 * 5 * 1.13 * max(1.0, float(plain.abs().max()))
