@@ -34,7 +34,7 @@ __device__ __forceinline__ void slope_vector(const Pack<T, VEC>& gy, const float
     for (int j = 0; j < VEC; ++j) g[j] = z[j] > 0.f ? g[j] : 0.f;
   } else {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) g[j] *= act_slope<AK>(z[j], act);
+    for (int j = 0; j < VEC; ++j) g[j] *= act_slope<AK, sizeof(T) == 4>(z[j], act);
   }
 }
 

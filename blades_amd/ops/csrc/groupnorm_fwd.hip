@@ -27,7 +27,7 @@ __device__ __forceinline__ void fwd_vector(const Pack<T, VEC>& x, size_t o, cons
   }
   V w;
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) from_f(act_f<AK>(z[j], act), w.e[j]);
+  for (int j = 0; j < VEC; ++j) from_f(act_f<AK, sizeof(T) == 4>(z[j], act), w.e[j]);
   store_out(y + o, w, through);
 }
 

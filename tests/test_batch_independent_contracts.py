@@ -149,3 +149,51 @@ def test_tensor_subclasses(dev, name):
     assert torch.equal(f([(2 * args[0]).as_subclass(Tagged)] + args[1:]).as_subclass(torch.Tensor), plain)
     got = f([Doubled(args[0])] + args[1:])
     assert float((got - plain).abs().max()) <= 2 * 512 * U32 * 5 * 1.13 * max(1.0, float(plain.abs().max()))
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# digits
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act,far", [("gelu", 12.0), ("silu", 80.0)])
+@pytest.mark.parametrize("C,groups", [(4096, 16), (4095, 15)])
+def test_activations_keep_their_digits(dev, act, far, C, groups, dt):
+    """Relative to the value, in the tails too.  A zero weight makes every channel's pre-activation its bias, exactly.
+
+    GELU, u a half step: the exponent z^2 / 2 is rounded twice and its factor once (1.25 z^2 u of e^(-z^2/2)), 2^x is off by
+    2 u, the reciprocal and its argument by 3 u, the polynomial by 3 u (fit) and 4 u (sums of up to twice the result), the
+    three products by 3 u: (16 + 1.5 z^2) u of the normal integral; within one standard deviation less than 9 u.  The
+    density: (4 + 1.25 z^2) u.  SiLU: 2^x and the reciprocal 2 u each, sums and products 4 u, 12 u with a margin; 16-bit
+    outputs |z| u more for the exponent.  Its slope s (1 + z (1 - s)) has these of s and of z s."""
+    z = torch.linspace(-far, far, C)
+    half, least = torch.finfo(dt).eps / 2, torch.finfo(dt).tiny * torch.finfo(dt).eps / 2
+    z64 = z.double()
+    if act == "gelu":
+        cdf, pdf = 0.5 * torch.special.erfc(-z64 / 2 ** 0.5), torch.exp(-z64 * z64 / 2) / (2 * torch.pi) ** 0.5
+        y, off = z64 * cdf, (16 + 1.5 * z64 * z64) * U32 * (z64 * cdf).abs()
+        slope, soff = cdf + z64 * pdf, (16 + 1.5 * z64 * z64) * U32 * (cdf + (z64 * pdf).abs())
+    else:
+        s, more = torch.sigmoid(z64), 0.0 if dt == torch.float32 else 2 * z64.abs()
+        y, off = z64 * s, (12 + more) * U32 * (z64 * s).abs()
+        slope, soff = s * (1 + z64 * (1 - s)), (24 + 2 * more) * U32 * s * (1 + z64.abs())
+    x = torch.randn(1, C, 3, device=dev).to(dt)
+    res = torch.zeros(1, C, 3, device=dev, dtype=dt).requires_grad_(True)
+    got = ops.group_norm(last(x), groups, torch.zeros(C, device=dev), z.to(dev), act=act, residual=last(res))
+    (g,) = torch.autograd.grad(got, res, torch.ones_like(got))
+    for a, want, tol in ((got, y, off), (g, slope, soff)):
+        err = (a[0].detach().double().cpu() - want.unsqueeze(1)).abs()
+        assert bool((err <= (tol + half * want.abs() + least).unsqueeze(1)).all()), float((err / want.abs().unsqueeze(1)).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
+def test_activations_of_infinities(dev, act):
+    """An infinity or NaN that the residual brings: as torch's activations of it in 64 bits (its 32-bit GELU on the CPU makes
+    an infinity NaN)."""
+    vals = torch.tensor([float("inf"), float("-inf"), float("nan"), 200.0, -200.0, 3e38, -3e38, 0.0])
+    x, w = torch.randn(1, 8, 4, device=dev), torch.zeros(8, device=dev)
+    res = vals.reshape(1, 8, 1).expand(1, 8, 4).contiguous()
+    got = ops.group_norm(last(x), 2, w, w, act=act, residual=last(res.to(dev))).cpu()
+    F = torch.nn.functional
+    want = {"none": lambda t: t, "relu": F.relu, "gelu": F.gelu, "silu": F.silu}[act](res.double()).float()
+    torch.testing.assert_close(got, want, rtol=16 * U32, atol=torch.finfo(torch.float32).tiny, equal_nan=True)
