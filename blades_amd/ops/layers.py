@@ -151,9 +151,9 @@ def client_dropout(x, uids, seed: int, tag, layer: int, p: float, kind: str = "e
 
 @functools.lru_cache(maxsize=256)
 def _draw(p: float):
-    """(smallest 24-bit draw that is kept, 1 / (1 - p)), both in 32 bits."""
-    p32 = c_float(p).value
-    return math.ceil(p32 * 16777216.0), c_float(1.0 / c_float(1.0 - p32).value).value
+    """(smallest 24-bit draw that is kept, 1 / (1 - p)): p rounded to 32 bits, as draws are compared with it, and the quotient
+    rounded to 32 bits once (from a rounded 1 - p it would be off by 1e-6 of itself at p = 0.99)."""
+    return math.ceil(c_float(p).value * 16777216.0), c_float(1.0 / (1.0 - p)).value
 
 
 def rope_axes(x, pos, axes, base: float = 10000.0, slots=None):

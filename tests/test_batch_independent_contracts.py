@@ -197,3 +197,23 @@ def test_activations_of_infinities(dev, act):
     F = torch.nn.functional
     want = {"none": lambda t: t, "relu": F.relu, "gelu": F.gelu, "silu": F.silu}[act](res.double()).float()
     torch.testing.assert_close(got, want, rtol=16 * U32, atol=torch.finfo(torch.float32).tiny, equal_nan=True)
+
+
+def check_scale(device, p):
+    y = ops.client_dropout(torch.ones(4000, device=device), torch.arange(1, device=device), 1, 1, 0, p)
+    kept = y[y != 0]
+    assert kept.numel() > 0 and bool((kept.double() * (1.0 - p) - 1.0).abs().max() <= U32 * (1 + 2 * U32))
+
+
+SCALES = [0.1, 0.3, 0.6, 0.701, 0.8, 0.9, 0.99, 0.999]
+
+
+@pytest.mark.parametrize("p", SCALES)
+def test_dropout_scale_is_rounded_once_cpu(p):
+    check_scale("cpu", p)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("p", SCALES)
+def test_dropout_scale_is_rounded_once(dev, p):
+    check_scale(dev, p)
