@@ -31,7 +31,7 @@ __device__ __forceinline__ void slope_vector(const Pack<T, VEC>& gy, const float
   }
   if (AK == 0 || (AK < 0 && act == 1)) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) g[j] = z[j] > 0.f ? g[j] : 0.f;
+    for (int j = 0; j < VEC; ++j) g[j] = z[j] <= 0.f ? 0.f : g[j];
   } else {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) g[j] *= act_slope<AK, sizeof(T) == 4>(z[j], act);

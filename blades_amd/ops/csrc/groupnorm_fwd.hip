@@ -22,7 +22,7 @@ __device__ __forceinline__ void fwd_vector(const Pack<T, VEC>& x, size_t o, cons
   if (gate != nullptr) {
     unsigned m = 0;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) m |= (z[j] > 0.f ? 1u : 0u) << j;
+    for (int j = 0; j < VEC; ++j) m |= (z[j] <= 0.f ? 0u : 1u) << j;  // (a NaN's gate is open: it was passed on)
     gate[o / VEC] = (unsigned char)m;
   }
   V w;

@@ -217,3 +217,32 @@ def test_dropout_scale_is_rounded_once_cpu(p):
 @pytest.mark.parametrize("p", SCALES)
 def test_dropout_scale_is_rounded_once(dev, p):
     check_scale(dev, p)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C,groups", [(8, 2), (6, 3)])
+@pytest.mark.parametrize("where", ["residual", "bias"])
+@pytest.mark.parametrize("pixels", [9, 200 * 211])  # in a workgroup's registers, in chunks
+def test_a_nan_passes_the_relu_both_ways(dev, where, pixels, C, groups):
+    """What is NaN in front of a ReLU comes out NaN, and its gradient passes, as torch has it."""
+    grads = []
+    for device, dt in (("cpu", torch.float64), (dev, torch.float32)):
+        g = torch.Generator().manual_seed(0)
+        x, r, gy = (torch.randn(2, C, pixels, generator=g) for _ in range(3))
+        b, w = torch.zeros(C), torch.ones(C)
+        r[0, 3, 5] = b[4] = float("nan")
+        leaves = [t.to(device=device, dtype=dt).requires_grad_(True) for t in (x, w, b if where == "bias" else 0 * w)]
+        res = r.to(device=device, dtype=dt).requires_grad_(True) if where == "residual" else None
+        y = ops.group_norm(last(leaves[0]), groups, leaves[1], leaves[2], act="relu", residual=None if res is None else last(res))
+        assert bool(y[:, 4].isnan().all()) if where == "bias" else int(y.isnan().sum()) == 1
+        grads.append([t.double().cpu() for t in torch.autograd.grad(
+            y, leaves + ([res] if res is not None else []), gy.to(device=device, dtype=dt))])
+    want, got = grads
+    if where == "residual":
+        assert float(want[3][0, 3, 5]) != 0.0 and torch.equal(got[3][0, 3, 5], want[3][0, 3, 5])
+        assert torch.equal(got[3].isnan(), want[3].isnan())
+    else:
+        # every gate of that channel is open: its sum of 2 * pixels gradients, of magnitude 0.8 on average
+        assert abs(float(got[2][4] - want[2][4])) <= 512 * U32 * 2 * pixels and abs(float(want[2][4])) > 0.1
+    for a, b in zip(got, want):
+        assert torch.equal(a.isnan(), b.isnan())
