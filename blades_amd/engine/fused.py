@@ -1013,17 +1013,34 @@ class _PCGroupNormFn(torch.autograd.Function):
 
 
 class PCGroupNorm(nn.Module):
+    """``act``: the activation directly behind it in its Sequential, which that one asks for with ``folded``; called by
+    anybody else the layer is the norm alone."""
+
     def __init__(self, gn: nn.GroupNorm, sink: GradSink, act: str = "none"):
         super().__init__()
         self.num_groups, self.eps, self.sink, self.act = gn.num_groups, gn.eps, sink, act
         self.weight, self.bias = gn.weight, gn.bias
 
     def extra_repr(self):
-        return f"{self.num_groups}, activation_folded={self.act}"
+        return f"{self.num_groups}, activation_behind={self.act}"
 
-    def forward(self, x, residual=None, relu: bool = False):
+    def forward(self, x, residual=None, relu: bool = False, folded: bool = False):
         anchor = self.weight if self.weight is not None else x
-        return _PCGroupNormFn.apply(x, residual, anchor, self, "relu" if relu else self.act)
+        return _PCGroupNormFn.apply(x, residual, anchor, self, "relu" if relu else self.act if folded else "none")
+
+
+class PCSequential(nn.Sequential):
+    """A Sequential that runs a group norm and the activation directly behind it as one kernel.  Both stay modules of their
+    own, so a model that calls, slices or walks the children itself gets what they compute."""
+
+    def forward(self, x):
+        kids = list(self._modules.values())
+        i = 0
+        while i < len(kids):
+            fold = i + 1 < len(kids) and type(kids[i]) is PCGroupNorm and _behind_group_norm(kids[i + 1]) == kids[i].act
+            x = kids[i](x, folded=True) if fold else kids[i](x)
+            i += 2 if fold else 1
+        return x
 
 
 def _conv_bn(conv, bn, x, residual=None, relu: bool = False, join=None, sole: bool = False):
@@ -1129,6 +1146,13 @@ def _cct_attention():
 _GN_ACTS = {nn.ReLU: "relu", nn.GELU: "gelu", nn.SiLU: "silu"}
 
 
+def _behind_group_norm(m: nn.Module):
+    """The activation that a group norm in front of ``m`` can take along, or None."""
+    if type(m) is PCActivation:
+        return m.kind
+    return _GN_ACTS.get(type(m)) if getattr(m, "approximate", "none") == "none" else None
+
+
 def build_template(model: nn.Module, sink: GradSink) -> nn.Module:
     memo = {id(p): p for p in model.parameters()}
     tmpl = copy.deepcopy(model, memo)
@@ -1142,14 +1166,14 @@ def build_template(model: nn.Module, sink: GradSink) -> nn.Module:
                     setattr(mod, n0, nn.Identity())
                     setattr(mod, n1, PCMaxPool2d(c1, relu=True))
         if type(mod) is nn.Sequential:
-            # an activation directly behind a group norm: folded into its kernel (a module that stands in several places
-            # is listed at each of them here)
+            # an activation directly behind a group norm (a module that stands in several places is listed at each of them
+            # here): PCSequential runs both in one kernel
             kids = list(mod._modules.items())
             for (n0, c0), (n1, c1) in zip(kids, kids[1:]):
-                act = _GN_ACTS.get(type(c1)) if type(c0) is nn.GroupNorm else None
-                if act is not None and getattr(c1, "approximate", "none") == "none":
+                act = _behind_group_norm(c1) if type(c0) is nn.GroupNorm else None
+                if act is not None:
                     setattr(mod, n0, PCGroupNorm(c0, sink, act))
-                    setattr(mod, n1, nn.Identity())
+                    mod.__class__ = PCSequential
         for name, child in list(mod.named_children()):
             if isinstance(child, nn.Conv2d):
                 setattr(mod, name, PCConv2d(child, sink))

@@ -1,6 +1,7 @@
 """What callers may ask of group norm, client-keyed dropout and rotary positions besides their values."""
 import pytest
 import torch
+from torch import nn
 from torch.autograd import forward_ad
 
 from blades_amd import ops
@@ -246,3 +247,35 @@ def test_a_nan_passes_the_relu_both_ways(dev, where, pixels, C, groups):
         assert abs(float(got[2][4] - want[2][4])) <= 512 * U32 * 2 * pixels and abs(float(want[2][4])) > 0.1
     for a, b in zip(got, want):
         assert torch.equal(a.isnan(), b.isnan())
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# the engine's modules
+class Tapped(nn.Module):
+    """Calls, slices and walks the children of a Sequential besides running it."""
+
+    def __init__(self):
+        super().__init__()
+        self.body = nn.Sequential(nn.Conv2d(3, 8, 1), nn.GroupNorm(2, 8), nn.SiLU(), nn.Conv2d(8, 8, 1), nn.GroupNorm(4, 8),
+                                  nn.ReLU())
+
+    def forward(self, x):
+        h = self.body[1](self.body[0](x))  # in front of the activation
+        a = self.body[2](h) + 3 * h
+        b = self.body[:2](x)
+        c = self.body[0:5:4](x)            # the convolution and the second norm
+        d = x
+        for m in self.body:
+            d = m(d)
+        return torch.cat([a, b, c, d, self.body(x)], 1)
+
+
+def test_a_models_own_use_of_a_sequentials_children():
+    from blades_amd.engine.fused import GradSink, build_template
+
+    net, sink = Tapped(), GradSink()
+    sink.Kc = 2
+    tmpl = build_template(net, sink)
+    x = torch.randn(4, 3, 5, 5)
+    with torch.no_grad():
+        torch.testing.assert_close(tmpl(x), net(x), rtol=1e-5, atol=1e-5)
