@@ -1174,7 +1174,9 @@ def build_template(model: nn.Module, sink: GradSink) -> nn.Module:
                 if act is not None:
                     setattr(mod, n0, PCGroupNorm(c0, sink, act))
                     mod.__class__ = PCSequential
-        for name, child in list(mod.named_children()):
+        for name, child in list(mod._modules.items()):  # (a module that stands in several places: at each of them)
+            if child is None:
+                continue
             if isinstance(child, nn.Conv2d):
                 setattr(mod, name, PCConv2d(child, sink))
             elif isinstance(child, nn.Linear):

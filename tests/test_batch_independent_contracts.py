@@ -6,6 +6,7 @@ from torch.autograd import forward_ad
 
 from blades_amd import ops
 from blades_amd.ops import reference as ref
+from tests.test_engine_paths import build, one_round_updates
 
 U32 = 2.0 ** -24  # half a step of fp32, relative
 
@@ -279,3 +280,25 @@ def test_a_models_own_use_of_a_sequentials_children():
     x = torch.randn(4, 3, 5, 5)
     with torch.no_grad():
         torch.testing.assert_close(tmpl(x), net(x), rtol=1e-5, atol=1e-5)
+
+
+class Tied(nn.Module):
+    """One group norm in several places, with and without an activation behind it."""
+
+    def __init__(self):
+        super().__init__()
+        gn = nn.GroupNorm(2, 8)
+        self.body = nn.Sequential(nn.Conv2d(3, 8, 1), gn, nn.Conv2d(8, 8, 1), gn, nn.Conv2d(8, 8, 1), gn, nn.SiLU())
+        self.fc = nn.Linear(8, 10)
+
+    def forward(self, x):
+        return self.fc(self.body(x).mean((2, 3)))
+
+
+def test_a_group_norm_in_several_places(data_root):
+    """Its gradients are the sum over the places."""
+    a, b = build(data_root, Tied, "fused"), build(data_root, Tied, "vmap")
+    assert a.engine.fused is not None and b.engine.fused is None
+    Ua, Ub = one_round_updates(a)[0], one_round_updates(b)[0]
+    # two fp32 paths of under 100 operations in a chain, each off by under 16 half steps of its scale
+    assert float(((Ua - Ub).norm(dim=1) / Ub.norm(dim=1)).max()) < 1e-4
