@@ -1116,7 +1116,7 @@ def supports(model: nn.Module) -> bool:
             continue
         if isinstance(m, nn.BatchNorm2d) and not m.track_running_stats:
             continue
-        if isinstance(m, (nn.LayerNorm, nn.GroupNorm)):
+        if isinstance(m, nn.LayerNorm) or type(m) is nn.GroupNorm:  # (a subclass may have a forward of its own)
             continue
         if _broadcast_params(m) is not None:
             continue
@@ -1185,7 +1185,7 @@ def build_template(model: nn.Module, sink: GradSink) -> nn.Module:
                 setattr(mod, name, PCBatchNorm2d(child, sink))
             elif isinstance(child, nn.LayerNorm):
                 setattr(mod, name, PCLayerNorm(child, sink))
-            elif isinstance(child, nn.GroupNorm):
+            elif type(child) is nn.GroupNorm:
                 setattr(mod, name, PCGroupNorm(child, sink))
             elif isinstance(child, nn.MaxPool2d):
                 setattr(mod, name, PCMaxPool2d(child, relu=False))

@@ -302,3 +302,15 @@ def test_a_group_norm_in_several_places(data_root):
     Ua, Ub = one_round_updates(a)[0], one_round_updates(b)[0]
     # two fp32 paths of under 100 operations in a chain, each off by under 16 half steps of its scale
     assert float(((Ua - Ub).norm(dim=1) / Ub.norm(dim=1)).max()) < 1e-4
+
+
+def test_a_group_norm_with_a_forward_of_its_own_keeps_it():
+    """A subclass may compute something else: the fused executor leaves its model to the general path."""
+    from blades_amd.engine.fused import supports
+
+    class NormAct(nn.GroupNorm):
+        def forward(self, x):
+            return torch.tanh(super().forward(x))
+
+    assert supports(nn.Sequential(nn.Conv2d(3, 8, 1), nn.GroupNorm(2, 8)))
+    assert not supports(nn.Sequential(nn.Conv2d(3, 8, 1), NormAct(2, 8)))
