@@ -90,10 +90,10 @@ class ResNet(nn.Module):
         self.layer4 = self._stage(block, 512, num_blocks[3], 2, make_norm)
         self.linear = nn.Linear(512 * block.expansion, num_classes)
 
-    def _stage(self, block, planes, n, stride, norm):
-        blocks = []
+    def _stage(self, block, planes, n, stride, norm=_bn):
+        blocks, choice = [], {} if norm is _bn else {"norm": norm}  # (a block need not know of norms to have the default one)
         for s in [stride] + [1] * (n - 1):
-            blocks.append(block(self.in_planes, planes, s, norm))
+            blocks.append(block(self.in_planes, planes, s, **choice))
             self.in_planes = planes * block.expansion
         return nn.Sequential(*blocks)
 

@@ -314,3 +314,17 @@ def test_a_group_norm_with_a_forward_of_its_own_keeps_it():
 
     assert supports(nn.Sequential(nn.Conv2d(3, 8, 1), nn.GroupNorm(2, 8)))
     assert not supports(nn.Sequential(nn.Conv2d(3, 8, 1), NormAct(2, 8)))
+
+
+def test_a_residual_block_without_a_norm_argument():
+    """Blocks written for (in_planes, planes, stride) build a ResNet as they did before there was a choice of norm."""
+    from blades_amd.models.resnet import BasicBlock, ResNet
+
+    class Block(BasicBlock):
+        def __init__(self, in_planes, planes, stride=1):
+            super().__init__(in_planes, planes, stride)
+
+    net = ResNet(Block, [1, 1, 1, 1])
+    assert net(torch.randn(2, 3, 32, 32)).shape == (2, 10)
+    with pytest.raises(TypeError):
+        ResNet(Block, [1, 1, 1, 1], norm="group")
