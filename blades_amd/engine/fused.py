@@ -775,7 +775,7 @@ class PCAttention(nn.Module):
         self.attn_drop = attn.attn_drop
         self.proj = attn.proj
         self.proj_drop = attn.proj_drop
-        self.rope = attn.rope
+        self.rope = getattr(attn, "rope", None)
 
     def _drop_cfg(self):
         d = self.attn_drop

@@ -66,8 +66,9 @@ class Attention(nn.Module):
     def forward(self, x):
         B, N, C = x.shape
         qkv = self.qkv(x).reshape(B, N, 3, self.num_heads, C // self.num_heads)
-        if self.rope is not None:
-            qkv = self.rope(qkv)
+        rope = getattr(self, "rope", None)  # (modules pickled before there were rotary positions have none)
+        if rope is not None:
+            qkv = rope(qkv)
         q, k, v = qkv.permute(2, 0, 3, 1, 4)
         attn = self.attn_drop(((q @ k.transpose(-2, -1)) * self.scale).softmax(dim=-1))
         return self.proj_drop(self.proj((attn @ v).transpose(1, 2).reshape(B, N, C)))

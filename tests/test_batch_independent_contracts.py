@@ -328,3 +328,17 @@ def test_a_residual_block_without_a_norm_argument():
     assert net(torch.randn(2, 3, 32, 32)).shape == (2, 10)
     with pytest.raises(TypeError):
         ResNet(Block, [1, 1, 1, 1], norm="group")
+
+
+def test_an_attention_from_before_rotary_positions():
+    """Pickled by an earlier version: no position module, and none is asked for."""
+    from blades_amd.engine.fused import GradSink, PCAttention
+    from blades_amd.models.cctnets.layers import Attention
+
+    new = Attention(16, 2).eval()
+    old = Attention(16, 2).eval()
+    old.load_state_dict(new.state_dict())
+    del old.rope
+    x = torch.randn(2, 5, 16)
+    with torch.no_grad():
+        assert torch.equal(old(x), new(x)) and PCAttention(old, GradSink()).rope is None
