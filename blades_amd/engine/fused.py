@@ -953,7 +953,7 @@ class _PCGroupNormFn(torch.autograd.Function):
     kernel does not take, and the CPU, run the oracle, the backward pass through autograd on it."""
 
     @staticmethod
-    def forward(ctx, x, res, anchor, mod, act):
+    def forward(ctx, x, res, anchor, mod, act, train):
         sink: GradSink = mod.sink
         w, b = sink.param(mod.weight), sink.param(mod.bias)
         ctx.mod, ctx.act, ctx.has_res = mod, act, res is not None
@@ -962,7 +962,7 @@ class _PCGroupNormFn(torch.autograd.Function):
         if ctx.hip:
             w, b = (t if t is None else t.detach().float() for t in (w, b))
             y, stats, gate, plan = _hipmod().group_norm_forward(x, mod.num_groups, w, b, mod.eps, act, res, Kc,
-                                                                for_backward=any(ctx.needs_input_grad))
+                                                                for_backward=train and any(ctx.needs_input_grad))
             ctx.plan, ctx.affine = plan, (w, b)
             ctx.save_for_backward(x, res if act in ("gelu", "silu") else None, stats, gate)
             return y
@@ -991,7 +991,7 @@ class _PCGroupNormFn(torch.autograd.Function):
             dx, dres = _hipmod().group_norm_backward(x, gy.to(x.dtype), mod.num_groups, w, b, stats, ctx.plan, act, res, gate,
                                                      Kc, want_dx, want_dres and act != "none", dw, db, ld,
                                                      None if dw is None else sink.scale, acc)
-            return dx, (gy if act == "none" else dres) if want_dres else None, None, None, None
+            return dx, (gy if act == "none" else dres) if want_dres else None, None, None, None, None
         from blades_amd.ops import reference as ref
 
         x, res = ctx.saved_tensors
@@ -1009,7 +1009,7 @@ class _PCGroupNormFn(torch.autograd.Function):
         if mod.weight is not None:
             sink.write(mod.weight, got[id(w)])
             sink.write(mod.bias, got[id(b)])
-        return got[id(xs)] if want_dx else None, got[id(rs)] if want_dres else None, None, None, None
+        return got[id(xs)] if want_dx else None, got[id(rs)] if want_dres else None, None, None, None, None
 
 
 class PCGroupNorm(nn.Module):
@@ -1026,7 +1026,9 @@ class PCGroupNorm(nn.Module):
 
     def forward(self, x, residual=None, relu: bool = False, folded: bool = False):
         anchor = self.weight if self.weight is not None else x
-        return _PCGroupNormFn.apply(x, residual, anchor, self, "relu" if relu else self.act if folded else "none")
+        # (a Function's needs_input_grad is true under no_grad as well: the mode is asked for here)
+        return _PCGroupNormFn.apply(x, residual, anchor, self, "relu" if relu else self.act if folded else "none",
+                                    torch.is_grad_enabled())
 
 
 class PCSequential(nn.Sequential):

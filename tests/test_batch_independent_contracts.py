@@ -342,3 +342,26 @@ def test_an_attention_from_before_rotary_positions():
     x = torch.randn(2, 5, 16)
     with torch.no_grad():
         assert torch.equal(old(x), new(x)) and PCAttention(old, GradSink()).rope is None
+
+
+@pytest.mark.gpu
+def test_evaluation_stores_nothing_for_a_backward_pass(dev, monkeypatch):
+    from blades_amd.engine.fused import GradSink, PCGroupNorm
+
+    h, asked = ops._h(), []
+    forward = h.group_norm_forward
+
+    def spy(*a, **k):
+        out = forward(*a, **k)
+        asked.append((k["for_backward"], out[1] is not None or out[2] is not None))
+        return out
+
+    monkeypatch.setattr(h, "group_norm_forward", spy)
+    sink = GradSink()
+    sink.Kc = 1
+    m = PCGroupNorm(nn.GroupNorm(2, 8).to(dev), sink)
+    x = torch.randn(2, 8, 3, 3, device=dev)
+    with torch.no_grad():
+        y = m(x, residual=x, relu=True)
+    z = m(x, residual=x, relu=True)
+    assert asked == [(False, False), (True, True)] and torch.equal(y, z) and z.requires_grad
