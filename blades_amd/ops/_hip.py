@@ -85,9 +85,9 @@ def _affine(t, Kc: int, C: int, device, name: str):
     return _vec(t, C, device, name=name), 0
 
 
-# Workspaces and outputs of the kernels come from here.  BLADES_POISON=1 fills them with NaN / 0xFF first: a kernel
-# that reads a byte nothing wrote then shows up as a non-finite result instead of depending on what the allocator
-# handed out (tools/probes/poison_probe.py).
+# Workspaces and outputs of the kernels come from here, those of csrc/autograd.cpp's nodes from its `fresh`.
+# BLADES_POISON=1 fills them with NaN / 0xFF first: a kernel that reads a byte nothing wrote then shows up as a non-finite
+# result instead of depending on what the allocator handed out (tools/probes/poison_probe.py).
 import os as _os
 
 _POISON = _os.environ.get("BLADES_POISON") == "1"
@@ -1814,6 +1814,7 @@ def autograd():
         m = importlib.import_module("blades_amd.ops._autograd")
         m.entries([ctypes.cast(f, c_void_p).value for f in (_gn_plan_size, _gn_plan_fill, _gn_fwd, _gn_bwd, _client_drop,
                                                             _rope_plan_size, _rope_plan_fill, _rope)])
+        m.poison(_POISON)
         _autograd = m
     return _autograd
 

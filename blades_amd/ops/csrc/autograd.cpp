@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
 
+#include <cmath>
 #include <memory>
 #include <vector>
 
@@ -51,6 +52,13 @@ bool like(const Tensor& t, const Tensor& r) {
   return !t.defined() || (t.sizes() == r.sizes() && t.scalar_type() == r.scalar_type() && t.device() == r.device());
 }
 
+// Outputs and workspaces pass through here: filled with NaN / 0xFF first where that is asked for (BLADES_POISON, see _hip.py).
+bool poison = false;
+Tensor fresh(Tensor t) {
+  if (poison && t.numel() > 0) t.is_floating_point() ? t.fill_(NAN) : t.fill_(0xFF);
+  return t;
+}
+
 bool needs_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
 bool channels_last(const Tensor& t) {
@@ -62,11 +70,11 @@ Tensor to_channels_last(const Tensor& t) {
 }
 Tensor like_channels_last(const Tensor& x) {
   Tensor y = at::empty_like(x);
-  if (channels_last(y)) return y;
+  if (channels_last(y)) return fresh(y);
   std::vector<int64_t> s{x.size(0)};
   for (int64_t i = 2; i < x.dim(); ++i) s.push_back(x.size(i));
   s.push_back(x.size(1));
-  return at::empty(s, x.options()).movedim(-1, 1);
+  return fresh(at::empty(s, x.options())).movedim(-1, 1);
 }
 
 // A graph of a backward pass is only built to differentiate it again: its results then raise when that happens.
@@ -166,10 +174,10 @@ variable_list GroupNormBackward::apply(variable_list&& grads) {
     const auto f32 = x_.options().dtype(at::kFloat);
     const bool own_dres = nr && p->act != 0;
     if (nx) out[0] = like_channels_last(x_);
-    if (nw) out[1] = at::empty(w_.sizes(), f32);
-    if (nb) out[2] = at::empty(b_.sizes(), f32);
+    if (nw) out[1] = fresh(at::empty(w_.sizes(), f32));
+    if (nb) out[2] = fresh(at::empty(b_.sizes(), f32));
     if (own_dres) out[3] = like_channels_last(x_);
-    Tensor ws = at::empty({p->ws[1]}, x_.options().dtype(at::kByte));
+    Tensor ws = fresh(at::empty({p->ws[1]}, x_.options().dtype(at::kByte)));
     lib.gn_bwd(ptr(x_), ptr(r_), ptr(g_), ptr(gt), ptr<float>(w_), ptr<float>(b_), ptr<float>(st), ptr(out[0]), ptr(out[3]),
                nullptr, ptr<float>(out[1]), ptr<float>(out[2]), x_.size(1), 0, ptr<float>(ws), p->plan.data(), stream_of(x_));
     if (nr && !own_dres) out[3] = gy;
@@ -195,10 +203,10 @@ Tensor group_norm(const Tensor& x, int64_t groups, const MaybeTensor& weight, co
     w_ = affine(wt); b_ = affine(bs);
     g->make(x_, w_, b_, x_.size(1) % 4 == 0 && aligned(x_, r_, none) ? 4 : 1);
     y = like_channels_last(x_);
-    if (grad || g->ws[0]) stats = at::empty({2, x_.size(0), groups}, x_.options().dtype(at::kFloat));
-    if (grad && r_.defined() && act == 1) gate = at::empty({x_.numel() / g->vec}, x_.options().dtype(at::kByte));
+    if (grad || g->ws[0]) stats = fresh(at::empty({2, x_.size(0), groups}, x_.options().dtype(at::kFloat)));
+    if (grad && r_.defined() && act == 1) gate = fresh(at::empty({x_.numel() / g->vec}, x_.options().dtype(at::kByte)));
     Tensor ws;
-    if (g->ws[0]) ws = at::empty({g->ws[0]}, x_.options().dtype(at::kByte));
+    if (g->ws[0]) ws = fresh(at::empty({g->ws[0]}, x_.options().dtype(at::kByte)));
     lib.gn_fwd(ptr(x_), ptr(r_), ptr<float>(w_), ptr<float>(b_), ptr(y), ptr(gate), ptr<float>(stats), ptr<float>(ws),
                g->plan.data(), stream_of(x_));
   }
@@ -236,7 +244,7 @@ Tensor drop(const Tensor& t, const Tensor& uids, const Tensor& tag, long tag_val
     p.last = x.dim() == 4 && x.is_contiguous(at::MemoryFormat::ChannelsLast);
     if (!p.last) x = x.contiguous();
   }
-  Tensor y = at::empty_like(x);
+  Tensor y = fresh(at::empty_like(x));
   const int rc = lib.dropout(ptr(x), ptr(y), ptr<long>(uids), ptr<long>(tag), tag_value, &p, stream_of(x));
   if (rc != 0)
     throw py::value_error("client_dropout: rejected: a client's share of a layer has at most 1.7e10 elements (and at most 2^30 "
@@ -324,7 +332,7 @@ std::shared_ptr<std::vector<char>> rope_plan(const Tensor& x, const Tensor& pos,
 
 Tensor turn(const Tensor& t, const Tensor& pos, const Rope& r, int inverse) {
   const c10::DeviceGuard guard(t.device());
-  if (t.numel() == 0) return at::empty(t.sizes(), t.options());
+  if (t.numel() == 0) return fresh(at::empty(t.sizes(), t.options()));
   check_saved("rope_axes", (pos.scalar_type() == at::kFloat || pos.scalar_type() == at::kLong) && pos.device() == t.device() &&
               (pos.dim() == 2 || (pos.dim() == 3 && pos.size(0) == t.size(0))) && pos.size(-2) == t.size(1) &&
               pos.size(-1) == (int64_t)r.axes.size());
@@ -339,7 +347,7 @@ Tensor turn(const Tensor& t, const Tensor& pos, const Rope& r, int inverse) {
     vec = at_() % 16 || step() % w || x.size(-1) % w ? 2 : w;
   }
   const auto plan = rope_plan(x, p, r, vec);
-  Tensor y = at::empty(x.sizes(), x.options());
+  Tensor y = fresh(at::empty(x.sizes(), x.options()));
   const int rc = lib.rope(ptr(x), ptr(y), ptr(p), plan->data(), inverse, stream_of(x));
   if (rc != 0) throw py::value_error("rope_axes: rejected (rc=" + std::to_string(rc) + ")");
   return y;
@@ -392,6 +400,7 @@ void entries(const std::vector<uintptr_t>& a) {
 
 PYBIND11_MODULE(_autograd, m) {
   m.def("entries", &entries);
+  m.def("poison", [](bool on) { poison = on; });
   m.def("group_norm", &group_norm);
   m.def("client_dropout", &client_dropout);
   m.def("rope_axes", &rope_axes);

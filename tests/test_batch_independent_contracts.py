@@ -365,3 +365,46 @@ def test_evaluation_stores_nothing_for_a_backward_pass(dev, monkeypatch):
         y = m(x, residual=x, relu=True)
     z = m(x, residual=x, relu=True)
     assert asked == [(False, False), (True, True)] and torch.equal(y, z) and z.requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", LAYERS)
+def test_poisoned_buffers(dev, name):
+    """Asked for poisoned buffers, the nodes fill every one they allocate, in both passes, and the results stay."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from blades_amd.ops import layers as mod
+
+    class Log(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.empty, self.filled = 0, 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.empty += func.overloadpacket in (torch.ops.aten.empty, torch.ops.aten.empty_like)
+            self.filled += func.overloadpacket is torch.ops.aten.fill_
+            return func(*args, **(kwargs or {}))
+
+    nodes, (f, args) = mod._nodes(), layers(dev)[name]
+    big = [last(torch.randn(2, 24, 130, 121, device=dev)) for _ in range(2)]  # a group norm in chunks: workspaces
+
+    def run():
+        leaves = [a.detach().clone(memory_format=torch.preserve_format).requires_grad_(True) for a in args]
+        y = f(leaves)
+        out = [y.detach(), *torch.autograd.grad(y, leaves, torch.ones_like(y))]
+        if name == "group_norm":
+            x = big[0].requires_grad_(True)
+            y = ops.group_norm(x, 1, act="relu", residual=big[1])
+            out += [y.detach(), *torch.autograd.grad(y, x, big[1])]
+        return out
+
+    plain = run()
+    try:
+        nodes.poison(True)
+        assert all(torch.equal(a, b) for a, b in zip(run(), plain))
+        with pytest.MonkeyPatch.context() as m, Log() as log:
+            m.setattr(mod, "_recorded", lambda: False)  # (the kernels, though somebody is listening)
+            run()
+    finally:
+        nodes.poison(False)
+    assert log.filled == log.empty >= (13 if name == "group_norm" else 2), (log.filled, log.empty)
