@@ -1865,8 +1865,6 @@ class _GnPlan:
         self.at, self.vec = ctypes.addressof(self.buf), vec
         ws = (c_long * 2)()
         rc = _gn_plan_fill(self.at, N, P, C, G, eps, act, per_client, gstride, bstride, dt, vec, ws)
-        if rc == 1:
-            raise ValueError("group_norm: rejected")
         self.ws = None if rc else (ws[0], ws[1])
 
 
@@ -1893,8 +1891,9 @@ def group_norm_plan(x, G, eps, act, clients, weight, bias, *others):
                     0 if weight is None or weight.dim() == 1 else weight.stride(0),
                     0 if bias is None or bias.dim() == 1 else bias.stride(0), _DT_CODE[x.dtype], vec)
     if plan.ws is None:
-        raise ValueError(f"group_norm: {C} channels in {G} groups over {x.numel() // (N * C)} pixels are not supported (a group "
-                         f"has at most 2048 channels; 1024 where C or an address rules out accesses of four)")
+        raise ValueError(f"group_norm: {N} samples of {C} channels in {G} groups over {x.numel() // (N * C)} pixels are not "
+                         f"supported (fewer than 2^24 samples, at most 2^24 channels, fewer than 2^30 pixels; a group has at "
+                         f"most 2048 channels, 1024 where C or an address rules out accesses of four)")
     return plan
 
 

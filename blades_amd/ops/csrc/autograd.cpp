@@ -112,9 +112,10 @@ struct GroupNorm {
     int rc = fill(v);
     if (rc == 2 && v > 1) rc = fill(1);  // wide groups of an odd number of channels
     if (rc != 0)
-      throw py::value_error("group_norm: " + std::to_string(C) + " channels in " + std::to_string(groups) + " groups over " +
-                            std::to_string(P) + " pixels are not supported (a group has at most 2048 channels; 1024 where C or "
-                            "an address rules out accesses of four)");
+      throw py::value_error("group_norm: " + std::to_string(N) + " samples of " + std::to_string(C) + " channels in " +
+                            std::to_string(groups) + " groups over " + std::to_string(P) + " pixels are not supported (fewer "
+                            "than 2^24 samples, at most 2^24 channels, fewer than 2^30 pixels; a group has at most 2048 "
+                            "channels, 1024 where C or an address rules out accesses of four)");
   }
 };
 

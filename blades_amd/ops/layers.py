@@ -80,8 +80,9 @@ def group_norm(x, groups: int, weight=None, bias=None, eps: float = 1e-5, act: s
 
     ``x [N, C, *]``, read channels last (other layouts are copied); ``weight`` / ``bias`` ``[C]``, or ``[K, C]``: one row
     for each of K clients that own N / K consecutive samples (their gradients then come per client).  ``act``: none, relu,
-    gelu (erf) or silu.  Statistics, products and sums are 32-bit, the result is rounded once.  A group has at most 2048
-    channels on the GPU (1024 where C or an address rules out accesses of four)."""
+    gelu (erf) or silu.  Statistics, products and sums are 32-bit, the result is rounded once.  On the GPU a group has
+    at most 2048 channels (1024 where C or an address rules out accesses of four), the layer at most 2^24 channels, fewer than
+    2^24 samples and fewer than 2^30 pixels."""
     if x.dim() < 2 or not x.is_floating_point():
         raise ValueError(f"group_norm: expected a floating-point tensor [N, C, *], got {x.dtype} {tuple(x.shape)}")
     N, C = x.shape[0], x.shape[1]

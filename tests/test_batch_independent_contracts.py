@@ -408,3 +408,22 @@ def test_poisoned_buffers(dev, name):
     finally:
         nodes.poison(False)
     assert log.filled == log.empty >= (13 if name == "group_norm" else 2), (log.filled, log.empty)
+
+
+@pytest.mark.gpu
+def test_more_samples_than_a_group_norm_takes(dev):
+    """Refused by the function, in words that name the limit; the engine's layer falls back to the oracle."""
+    from blades_amd.engine.fused import GradSink, PCGroupNorm
+
+    x = torch.zeros(1 << 24, 4, device=dev, dtype=torch.bfloat16)
+    x[-1] = torch.tensor([1.0, 3.0, -2.0, 2.0])
+    with pytest.raises(ValueError, match="samples"):
+        ops.group_norm(x, 2)
+    assert not ops._h().group_norm_supported(x, 2) and ops._h().group_norm_supported(x[1:], 2)
+    with pytest.raises(ValueError, match="2048 channels"):
+        ops.group_norm(torch.zeros(2, 2056, device=dev), 1)
+    assert not ops._h().group_norm_supported(torch.zeros(2, 2056, device=dev), 1)
+    sink = GradSink()
+    sink.Kc = 1
+    y = PCGroupNorm(nn.GroupNorm(2, 4, eps=0.0, affine=False), sink)(x)
+    assert y[-1].tolist() == [-1.0, 1.0, -1.0, 1.0]
