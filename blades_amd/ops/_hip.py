@@ -1864,7 +1864,7 @@ class _GnPlan:
         self.buf = ctypes.create_string_buffer(_gn_plan_size())
         self.at, self.vec = ctypes.addressof(self.buf), vec
         ws = (c_long * 2)()
-        rc = _gn_plan_fill(self.at, N, P, C, G, eps, act, per_client, gstride, bstride, dt, vec, ws)
+        rc = 1 if C > 1 << 24 else _gn_plan_fill(self.at, N, P, C, G, eps, act, per_client, gstride, bstride, dt, vec, ws)
         self.ws = None if rc else (ws[0], ws[1])
 
 
@@ -1987,6 +1987,8 @@ def _rope_plan(shape, stride, five, per_sample, pos_float, dtype, narrow, axes, 
     """(plan, its address): what a rope_axes launch's shape fixes."""
     R, N, H, D = shape[0], shape[1], shape[-2], shape[-1]
     dt = _DT_CODE[dtype]
+    if H * (shape[2] if five else 1) > 10 ** 9:  # (the plan's counts are ints)
+        raise ValueError("rope_axes: a token has at most 10^9 rows (slots times heads)")
     plan = ctypes.create_string_buffer(_rope_plan_size())
     rc = _rope_plan_fill(plan, pos_float, N * len(axes) if per_sample else 0, R, N, shape[2] if five else 1, H, D, stride[0],
                          stride[1], stride[2] if five else 0, stride[-2], slots, (c_int * len(axes))(*axes), len(axes), base, dt,

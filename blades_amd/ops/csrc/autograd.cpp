@@ -109,7 +109,7 @@ struct GroupNorm {
       return lib.gn_plan(plan.data(), N, P, (int)C, groups, eps, act, (int)(N / clients), strides[0], strides[1], dtype_of(x),
                          vec, ws);
     };
-    int rc = fill(v);
+    int rc = C > (1 << 24) ? 1 : fill(v);  // (the plan's counts are ints)
     if (rc == 2 && v > 1) rc = fill(1);  // wide groups of an odd number of channels
     if (rc != 0)
       throw py::value_error("group_norm: " + std::to_string(N) + " samples of " + std::to_string(C) + " channels in " +
@@ -316,6 +316,8 @@ std::shared_ptr<std::vector<char>> rope_plan(const Tensor& x, const Tensor& pos,
   static thread_local std::vector<std::pair<RopeKey, std::shared_ptr<std::vector<char>>>> kept;
   const bool five = x.dim() == 5;
   const long R = x.size(0), N = x.size(1), psr = pos.dim() == 3 ? N * (long)r.axes.size() : 0;
+  if ((double)x.size(-2) * (five ? x.size(2) : 1) > 1e9)  // (the plan's counts are ints)
+    throw py::value_error("rope_axes: a token has at most 10^9 rows (slots times heads)");
   const int S = five ? (int)x.size(2) : 1, H = (int)x.size(-2), D = (int)x.size(-1), dt = dtype_of(x);
   const int pf = pos.scalar_type() == at::kFloat;
   RopeKey key{{pf, psr, R, N, S, H, D, x.stride(0), x.stride(1), five ? x.stride(2) : 0, x.stride(-2), r.slots, dt, vec}, r.base};

@@ -164,7 +164,7 @@ def rope_axes(x, pos, axes, base: float = 10000.0, slots=None):
     all) are turned and whose others are copied.  ``axes``: even widths of the sections, one per axis, together at most D
     (the rest of the head passes through).  ``pos``: int64 or fp32 positions, ``[N, A]`` shared by the samples or
     ``[R, N, A]``.  Pair (2i, 2i + 1) of a section d wide is turned by ``pos * base ** (-2 i / d)``; angles are 64-bit.
-    D is even, at most 256; at most 8 axes."""
+    D is even, at most 256; at most 8 axes; on the GPU S * H is at most 10^9."""
     if x.dim() not in (4, 5) or not x.is_floating_point():
         raise ValueError(f"rope_axes: expected a floating-point [R, N, H, D] or [R, N, S, H, D] tensor, got {x.dtype} "
                          f"{tuple(x.shape)}")

@@ -427,3 +427,18 @@ def test_more_samples_than_a_group_norm_takes(dev):
     sink.Kc = 1
     y = PCGroupNorm(nn.GroupNorm(2, 4, eps=0.0, affine=False), sink)(x)
     assert y[-1].tolist() == [-1.0, 1.0, -1.0, 1.0]
+
+
+@pytest.mark.gpu
+def test_sizes_past_32_bits_are_refused(dev):
+    """Counts that an int of the plan would cut to a few channels or slots, leaving the rest of the output unwritten."""
+    with pytest.raises(ValueError, match="channels"):
+        ops.group_norm(torch.empty(1, 2 ** 32 + 4, device=dev, dtype=torch.float16), 1)
+    assert not ops._h().group_norm_supported(torch.empty(1, 2 ** 32 + 4, device=dev, dtype=torch.float16), 1)
+    pos = torch.zeros(1, 1, dtype=torch.int64, device=dev)
+    one = torch.zeros(1, 1, 1, 1, 2, device=dev, dtype=torch.float16)
+    for shape in ((1, 1, 2 ** 32 + 1, 1, 2), (1, 1, 1, 2 ** 32 + 1, 2)):
+        with pytest.raises(ValueError):
+            ops.rope_axes(one.expand(shape), pos, (2,))
+        with pytest.raises(ValueError):
+            ops._h().rope_axes(one.expand(shape), pos, (2,))
