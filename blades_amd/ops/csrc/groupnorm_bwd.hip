@@ -333,8 +333,8 @@ BLADES_API int blades_group_norm_backward(const void* x, const void* res, const 
 #undef GN_BT
 #undef GN_B
   if (dgamma != nullptr || dbeta != nullptr) {
+    // (samples times chunks stay below 2^24 + 2048: make_plan cuts samples only while there are fewer than 2048 workgroups)
     const long rows = (long)q.per_client * q.nchunk, clients = q.N / q.per_client;
-    if (rows >= (1L << 31)) return 1;
     const int groups = cdiv(q.C, CH);
     const long most = ((1L << 32) - 1) / ((long)groups * AFF_THREADS);  // a grid counts its threads in 32 bits
     for (long k = 0; k < clients; k += most) {

@@ -442,3 +442,29 @@ def test_sizes_past_32_bits_are_refused(dev):
             ops.rope_axes(one.expand(shape), pos, (2,))
         with pytest.raises(ValueError):
             ops._h().rope_axes(one.expand(shape), pos, (2,))
+
+
+def test_group_norm_plan_bounds_samples_times_chunks():
+    """The affine sums count a client's samples times chunks in 31 bits: below 2^24 + 2048 for every layer the plan takes (read
+    off the backward pass's workspace: samples x chunks x C entries of 8 bytes, and at most one per sample and group)."""
+    import ctypes
+    import random
+
+    from blades_amd.ops import build
+
+    if not build.HIP_LIB.exists():
+        pytest.skip("kernels are not built")
+    lib = ctypes.CDLL(str(build.HIP_LIB))
+    lib.blades_group_norm_plan_size.restype = ctypes.c_long
+    buf, ws = ctypes.create_string_buffer(lib.blades_group_norm_plan_size()), (ctypes.c_long * 2)()
+    L, I, rng, taken = ctypes.c_long, ctypes.c_int, random.Random(1), 0
+    for _ in range(4000):
+        C = int(2 ** rng.uniform(0, 12))
+        G = rng.choice([g for g in range(1, C + 1) if C % g == 0])
+        N, P = (int(2 ** rng.uniform(0, e)) for e in (24, 30))
+        dt = rng.randrange(3)
+        if lib.blades_group_norm_plan(buf, L(N), L(P), I(C), I(G), ctypes.c_float(1e-5), I(0), I(N), L(0), L(0), I(dt),
+                                      I(1 if C % 4 else 4), ws) == 0:
+            taken += 1
+            assert ws[1] // (8 * C) < (1 << 24) + 2048 + N  # (the means: at most N x G <= N x C entries)
+    assert taken > 2000
