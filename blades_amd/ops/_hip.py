@@ -1924,13 +1924,12 @@ def _gn_check(name, x, groups, clients, weight, bias, *others):
 
 
 def group_norm_forward(x, groups: int, weight, bias, eps: float, act: str = "none", residual=None, clients: int = 1,
-                       for_backward: bool = True, checked: bool = False):
+                       for_backward: bool = True):
     """``act(group_norm(x) * weight + bias + residual)`` for channels-last ``x [N, C, *]`` (fp32, bf16 or fp16).
     ``weight`` / ``bias``: fp32 ``[C]`` or ``[clients, C]`` (any client stride).  Returns (y, stats, gate, plan).  For a
     backward pass: stats ``[2, N, groups]`` (mean, 1 / std) and, for a ReLU behind a residual, its gate, one byte per vector,
-    which spares that pass the residual; else None.  ``checked``: the caller did."""
-    if not checked:
-        _gn_check("group_norm", x, groups, clients, weight, bias, residual)
+    which spares that pass the residual; else None."""
+    _gn_check("group_norm", x, groups, clients, weight, bias, residual)
     x = to_channels_last(x)
     residual = None if residual is None else to_channels_last(residual)
     plan = group_norm_plan(x, groups, eps, act, clients, weight, bias, residual)
@@ -1949,25 +1948,24 @@ def group_norm_forward(x, groups: int, weight, bias, eps: float, act: str = "non
 
 def group_norm_backward(x, gy, groups: int, weight, bias, stats, plan, act: str = "none", residual=None, gate=None,
                         clients: int = 1, want_dx: bool = True, want_dres: bool = False, dweight=None, dbias=None, ld: int = 0,
-                        coef=None, accumulate: bool = False, checked: bool = False):
+                        coef=None, accumulate: bool = False):
     """Gradients of ``group_norm_forward``, whose ``stats``, ``gate`` and ``plan`` these are: returns (dx, dres).
     ``dweight`` / ``dbias``: fp32 ``[clients, C]`` tensors, rows ``ld`` floats apart (columns of the update matrix, for one);
     they receive — ``accumulate``: are incremented by — ``coef[client]`` (None: 1) times the sums.  ``gate`` stands in for the
     residual."""
-    if not checked:
-        _gn_check("group_norm_backward", x, groups, clients, weight, bias, gy, residual)
-        N, C = x.shape[0], x.shape[1]
-        if stats.device != x.device or stats.dtype != torch.float32 or not stats.is_contiguous() \
-                or stats.numel() != 2 * N * groups:
-            raise ValueError("group_norm_backward: stats do not match")
-        for n, t in (("dweight", dweight), ("dbias", dbias)):
-            if t is not None and not (t.device == x.device and t.dtype == torch.float32 and tuple(t.shape) == (clients, C)
-                                      and t.stride(1) == 1 and (clients == 1 or t.stride(0) == ld) and ld >= C):
-                raise ValueError(f"group_norm_backward: {n} must be fp32 [{clients}, {C}] with row stride ld")
-        if coef is not None:
-            coef = _vec(coef, clients, x.device, name="coef")
-        if gate is not None and (gate.numel() * plan.vec != x.numel() or gate.device != x.device):
-            raise ValueError("group_norm_backward: the gate does not match x")
+    _gn_check("group_norm_backward", x, groups, clients, weight, bias, gy, residual)
+    N, C = x.shape[0], x.shape[1]
+    if stats.device != x.device or stats.dtype != torch.float32 or not stats.is_contiguous() \
+            or stats.numel() != 2 * N * groups:
+        raise ValueError("group_norm_backward: stats do not match")
+    for n, t in (("dweight", dweight), ("dbias", dbias)):
+        if t is not None and not (t.device == x.device and t.dtype == torch.float32 and tuple(t.shape) == (clients, C)
+                                  and t.stride(1) == 1 and (clients == 1 or t.stride(0) == ld) and ld >= C):
+            raise ValueError(f"group_norm_backward: {n} must be fp32 [{clients}, {C}] with row stride ld")
+    if coef is not None:
+        coef = _vec(coef, clients, x.device, name="coef")
+    if gate is not None and (gate.numel() * plan.vec != x.numel() or gate.device != x.device):
+        raise ValueError("group_norm_backward: the gate does not match x")
     x, gy = to_channels_last(x), to_channels_last(gy)
     residual = None if residual is None or gate is not None else to_channels_last(residual)
     if plan.vec > 1:  # the forward pass's accesses, and its gate's
@@ -1998,27 +1996,25 @@ def _rope_plan(shape, stride, five, per_sample, pos_float, dtype, narrow, axes, 
     return plan, ctypes.addressof(plan)
 
 
-def rope_axes(x, pos, axes, base: float = 10000.0, slots=None, inverse: bool = False, out=None, checked: bool = False):
+def rope_axes(x, pos, axes, base: float = 10000.0, slots=None, inverse: bool = False, out=None):
     """Rotary positions with several axes (see reference.rope_axes).  ``x`` may have any strides (last dimension
-    contiguous).  ``out``: None for a new contiguous tensor, or ``x`` itself: turned in place, other slots untouched.
-    ``checked``: the caller did, and ``axes`` is a tuple of ints, ``slots`` an int."""
+    contiguous).  ``out``: None for a new contiguous tensor, or ``x`` itself: turned in place, other slots untouched."""
     shape, five = x.shape, x.dim() == 5
-    if not checked:
-        R, N, D, S = shape[0], shape[1], shape[-1], shape[2] if five else 1
-        axes, slots = tuple(int(a) for a in axes), S if slots is None else int(slots)
-        if not (x.is_cuda and x.dtype in _DT_CODE and x.dim() in (4, 5)):
-            raise ValueError(f"rope_axes: expected a CUDA fp32 / bf16 / fp16 tensor [R, N, H, D] or [R, N, S, H, D], got "
-                             f"{x.device} {x.dtype} {tuple(shape)}")
-        if not axes or len(axes) > 8 or any(a < 2 or a % 2 for a in axes) or sum(axes) > D or D % 2 or D > 256:
-            raise ValueError(f"rope_axes: sections {axes} must be even and fit the head dimension {D} (even, at most 256)")
-        if not 0 <= slots <= S or not base > 0.0:
-            raise ValueError(f"rope_axes: {slots} of {S} slots, base {base}")
-        if pos.device != x.device or pos.dtype not in (torch.int64, torch.float32) or tuple(pos.shape) not in (
-                (N, len(axes)), (R, N, len(axes))):
-            raise ValueError(f"rope_axes: pos must be int64 or fp32 [{N}, {len(axes)}] or [{R}, {N}, {len(axes)}] on x's "
-                             f"device, got {pos.dtype} {tuple(pos.shape)} on {pos.device}")
-        if out is not None and (out is not x or x.stride(-1) != 1 or not _no_overlap(x)):
-            raise ValueError("rope_axes: out must be x itself, without overlapping elements, its last dimension contiguous")
+    R, N, D, S = shape[0], shape[1], shape[-1], shape[2] if five else 1
+    axes, slots = tuple(int(a) for a in axes), S if slots is None else int(slots)
+    if not (x.is_cuda and x.dtype in _DT_CODE and x.dim() in (4, 5)):
+        raise ValueError(f"rope_axes: expected a CUDA fp32 / bf16 / fp16 tensor [R, N, H, D] or [R, N, S, H, D], got "
+                         f"{x.device} {x.dtype} {tuple(shape)}")
+    if not axes or len(axes) > 8 or any(a < 2 or a % 2 for a in axes) or sum(axes) > D or D % 2 or D > 256:
+        raise ValueError(f"rope_axes: sections {axes} must be even and fit the head dimension {D} (even, at most 256)")
+    if not 0 <= slots <= S or not base > 0.0:
+        raise ValueError(f"rope_axes: {slots} of {S} slots, base {base}")
+    if pos.device != x.device or pos.dtype not in (torch.int64, torch.float32) or tuple(pos.shape) not in (
+            (N, len(axes)), (R, N, len(axes))):
+        raise ValueError(f"rope_axes: pos must be int64 or fp32 [{N}, {len(axes)}] or [{R}, {N}, {len(axes)}] on x's "
+                         f"device, got {pos.dtype} {tuple(pos.shape)} on {pos.device}")
+    if out is not None and (out is not x or x.stride(-1) != 1 or not _no_overlap(x)):
+        raise ValueError("rope_axes: out must be x itself, without overlapping elements, its last dimension contiguous")
     if not pos.is_contiguous():
         pos = pos.contiguous()
     if x.numel() == 0:
@@ -2037,7 +2033,7 @@ def rope_axes(x, pos, axes, base: float = 10000.0, slots=None, inverse: bool = F
             if out is not None:
                 raise ValueError("rope_axes: in place needs pairs at even addresses")
             x = x.clone(memory_format=torch.contiguous_format)
-            return rope_axes(x, pos, axes, base, slots, inverse, None, True)
+            return rope_axes(x, pos, axes, base, slots, inverse)
     plan = _rope_plan(shape, stride, five, pos.dim() == 3, pos.dtype == torch.float32, x.dtype, narrow, axes, base, slots)
     y = x if out is not None else _empty(shape, dtype=x.dtype, device=x.device)
     rc = _launch(x.device.index, _rope, at, y.data_ptr(), pos.data_ptr(), plan[1], inverse)
