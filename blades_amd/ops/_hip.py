@@ -1794,6 +1794,7 @@ _gn_plan_fill = _opt_sig("blades_group_norm_plan", [_P, c_long, c_long, c_int, c
                                                     c_int, c_int, _P], c_int)
 _gn_fwd = _opt_sig("blades_group_norm_forward", [_P] * 10, c_int)
 _gn_bwd = _opt_sig("blades_group_norm_backward", [_P] * 12 + [c_long, c_int] + [_P] * 3, c_int)
+_client_drop_plan_size = _opt_sig("blades_client_dropout_plan_size", [], c_long)
 _client_drop = _opt_sig("blades_client_dropout", [_P, _P, _P, _P, c_long, _P, _P], c_int)
 _rope_plan_size = _opt_sig("blades_rope_plan_size", [], c_long)
 _rope_plan_fill = _opt_sig("blades_rope_plan", [_P, c_int, c_long, c_long, c_long, c_int, c_int, c_int, c_long, c_long, c_long,
@@ -1812,8 +1813,9 @@ def autograd():
         import importlib
 
         m = importlib.import_module("blades_amd.ops._autograd")
-        m.entries([ctypes.cast(f, c_void_p).value for f in (_gn_plan_size, _gn_plan_fill, _gn_fwd, _gn_bwd, _client_drop,
-                                                            _rope_plan_size, _rope_plan_fill, _rope)])
+        m.entries([ctypes.cast(f, c_void_p).value for f in (
+            _gn_plan_size, _gn_plan_fill, _gn_fwd, _gn_bwd, _client_drop_plan_size, _client_drop, _rope_plan_size,
+            _rope_plan_fill, _rope)])
         m.poison(_POISON)
         _autograd = m
     return _autograd

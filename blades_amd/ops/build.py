@@ -94,7 +94,7 @@ def build_hip(force: bool = False, verbose: bool = False, jobs: int = 4) -> Path
 
 def build_autograd(force: bool = False, verbose: bool = False) -> Path:
     src = CSRC / "autograd.cpp"
-    if force or _stale(AUTOGRAD_LIB, [src]):
+    if force or _stale(AUTOGRAD_LIB, [src] + _headers(src)):
         import sysconfig
 
         import torch

@@ -17,6 +17,8 @@
 #include <memory>
 #include <vector>
 
+#include "layers_abi.h"
+
 namespace {
 
 using at::Tensor;
@@ -27,18 +29,18 @@ typedef std::optional<Tensor> MaybeTensor;
 
 // entry points of libblades_hip (see the sources for the arguments)
 struct {
-  long (*gn_plan_size)();
-  int (*gn_plan)(void*, long, long, int, int, float, int, int, long, long, int, int, long*);
-  int (*gn_fwd)(const void*, const void*, const float*, const float*, void*, void*, float*, float*, const void*, void*);
-  int (*gn_bwd)(const void*, const void*, const void*, const void*, const float*, const float*, const float*, void*, void*,
-                const float*, float*, float*, long, int, float*, const void*, void*);
-  int (*dropout)(const void*, void*, const long*, const long*, long, const void*, void*);
-  long (*rope_plan_size)();
-  int (*rope_plan)(void*, int, long, long, long, int, int, int, long, long, long, long, int, const int*, int, double, int, int);
-  int (*rope)(const void*, void*, const void*, const void*, int, void*);
+  decltype(&blades_group_norm_plan_size) gn_plan_size;
+  decltype(&blades_group_norm_plan) gn_plan;
+  decltype(&blades_group_norm_forward) gn_fwd;
+  decltype(&blades_group_norm_backward) gn_bwd;
+  decltype(&blades_client_dropout_plan_size) dropout_plan_size;
+  decltype(&blades_client_dropout) dropout;
+  decltype(&blades_rope_plan_size) rope_plan_size;
+  decltype(&blades_rope_plan) rope_plan;
+  decltype(&blades_rope_axes) rope;
 } lib;
 
-void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
 int dtype_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? 0 : t.scalar_type() == at::kBFloat16 ? 1 : 2; }
 
@@ -94,6 +96,7 @@ struct GroupNorm {
   long clients;
   float eps;
 
+  groupnorm::Layer* layer() { return reinterpret_cast<groupnorm::Layer*>(plan.data()); }
   static long stride(const Tensor& t) { return t.defined() && t.dim() == 2 ? t.stride(0) : 0; }
   bool affine_fits(const Tensor& t, const Tensor& x, long C) const {
     return !t.defined() || (t.scalar_type() == at::kFloat && t.device() == x.device() && t.dim() > 0 && t.size(-1) == C &&
@@ -106,7 +109,7 @@ struct GroupNorm {
     strides[0] = stride(w); strides[1] = stride(b);
     auto fill = [&](int channels) {
       vec = channels;
-      return lib.gn_plan(plan.data(), N, P, (int)C, groups, eps, act, (int)(N / clients), strides[0], strides[1], dtype_of(x),
+      return lib.gn_plan(layer(), N, P, (int)C, groups, eps, act, (int)(N / clients), strides[0], strides[1], dtype_of(x),
                          vec, ws);
     };
     int rc = C > (1 << 24) ? 1 : fill(v);  // (the plan's counts are ints)
@@ -180,7 +183,7 @@ variable_list GroupNormBackward::apply(variable_list&& grads) {
     if (own_dres) out[3] = like_channels_last(x_);
     Tensor ws = fresh(at::empty({p->ws[1]}, x_.options().dtype(at::kByte)));
     lib.gn_bwd(ptr(x_), ptr(r_), ptr(g_), ptr(gt), ptr<float>(w_), ptr<float>(b_), ptr<float>(st), ptr(out[0]), ptr(out[3]),
-               nullptr, ptr<float>(out[1]), ptr<float>(out[2]), x_.size(1), 0, ptr<float>(ws), p->plan.data(), stream_of(x_));
+               nullptr, ptr<float>(out[1]), ptr<float>(out[2]), x_.size(1), 0, ptr<float>(ws), p->layer(), stream_of(x_));
     if (nr && !own_dres) out[3] = gy;
     if (nw && w_type != at::kFloat) out[1] = out[1].to(w_type);
     if (nb && b_type != at::kFloat) out[2] = out[2].to(b_type);
@@ -209,7 +212,7 @@ Tensor group_norm(const Tensor& x, int64_t groups, const MaybeTensor& weight, co
     Tensor ws;
     if (g->ws[0]) ws = fresh(at::empty({g->ws[0]}, x_.options().dtype(at::kByte)));
     lib.gn_fwd(ptr(x_), ptr(r_), ptr<float>(w_), ptr<float>(b_), ptr(y), ptr(gate), ptr<float>(stats), ptr<float>(ws),
-               g->plan.data(), stream_of(x_));
+               g->layer(), stream_of(x_));
   }
   if (!grad) return y;
   auto node = std::shared_ptr<GroupNormBackward>(new GroupNormBackward(), torch::autograd::deleteNode);
@@ -226,14 +229,6 @@ Tensor group_norm(const Tensor& x, int64_t groups, const MaybeTensor& weight, co
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-struct DropPlan {  // as in dropout.hip
-  long B, C, HW;
-  unsigned long long seed;
-  int Kc, kind, inner, last, dtype;
-  unsigned c3, least;
-  float scale;
-};
-
 Tensor drop(const Tensor& t, const Tensor& uids, const Tensor& tag, long tag_value, DropPlan p) {
   check_saved("client_dropout", uids.numel() == p.Kc && uids.scalar_type() == at::kLong && uids.device() == t.device() &&
               uids.is_contiguous() && (!tag.defined() || (tag.numel() == 1 && tag.scalar_type() == at::kLong &&
@@ -325,7 +320,7 @@ std::shared_ptr<std::vector<char>> rope_plan(const Tensor& x, const Tensor& pos,
   for (auto& k : kept)
     if (k.first == key) return k.second;
   auto plan = std::make_shared<std::vector<char>>(lib.rope_plan_size());
-  const int rc = lib.rope_plan(plan->data(), pf, psr, R, N, S, H, D, x.stride(0), x.stride(1), five ? x.stride(2) : 0,
+  const int rc = lib.rope_plan(reinterpret_cast<rope::RopePlan*>(plan->data()), pf, psr, R, N, S, H, D, x.stride(0), x.stride(1), five ? x.stride(2) : 0,
                                x.stride(-2), r.slots, r.axes.data(), (int)r.axes.size(), r.base, dt, vec);
   if (rc != 0) throw py::value_error("rope_axes: rejected (rc=" + std::to_string(rc) + ")");
   if (kept.size() >= 16) kept.erase(kept.begin());
@@ -351,7 +346,7 @@ Tensor turn(const Tensor& t, const Tensor& pos, const Rope& r, int inverse) {
   }
   const auto plan = rope_plan(x, p, r, vec);
   Tensor y = fresh(at::empty(x.sizes(), x.options()));
-  const int rc = lib.rope(ptr(x), ptr(y), ptr(p), plan->data(), inverse, stream_of(x));
+  const int rc = lib.rope(ptr(x), ptr(y), ptr(p), reinterpret_cast<rope::RopePlan*>(plan->data()), inverse, stream_of(x));
   if (rc != 0) throw py::value_error("rope_axes: rejected (rc=" + std::to_string(rc) + ")");
   return y;
 }
@@ -393,9 +388,11 @@ Tensor rope_axes(const Tensor& x, const Tensor& pos, const std::vector<int>& axe
 }
 
 void entries(const std::vector<uintptr_t>& a) {
-  TORCH_CHECK(a.size() == 8, "eight entry points are expected");
-  void* to[] = {&lib.gn_plan_size, &lib.gn_plan, &lib.gn_fwd, &lib.gn_bwd, &lib.dropout, &lib.rope_plan_size, &lib.rope_plan,
-                &lib.rope};
+  TORCH_CHECK(a.size() == 9, "nine entry points are expected");
+  TORCH_CHECK(reinterpret_cast<decltype(lib.dropout_plan_size)>(a[4])() == (long)sizeof(DropPlan),
+              "the kernels' library is of another build: build again");
+  void* to[] = {&lib.gn_plan_size, &lib.gn_plan, &lib.gn_fwd, &lib.gn_bwd, &lib.dropout_plan_size, &lib.dropout,
+                &lib.rope_plan_size, &lib.rope_plan, &lib.rope};
   for (size_t i = 0; i < a.size(); ++i) *static_cast<uintptr_t*>(to[i]) = a[i];
 }
 

@@ -12,6 +12,7 @@
 //
 // Multiplication, not selection, as the stored multipliers had it: 0 * inf stays NaN.
 #include "common.h"
+#include "layers_abi.h"
 
 namespace {
 constexpr int TPB = 256;
@@ -368,16 +369,7 @@ int dropout_t(const Key& key, const void* x, void* y, int Kc, long B, long C, lo
 }
 }  // namespace
 
-// What a layer's shape and key fix.  dtype 0 fp32, 1 bf16, 2 fp16.  kind 0 element, 1 channel, 2 sample.  last: channels-last
-// maps, else contiguous [.., C, HW].  inner: [B][Kc][C] instead of [Kc][B][C] in the leading dimensions.  least: smallest
-// 24-bit draw that is kept, below 2^24.
-struct DropPlan {
-  long B, C, HW;
-  unsigned long long seed;
-  int Kc, kind, inner, last, dtype;
-  unsigned c3, least;
-  float scale;
-};
+BLADES_API long blades_client_dropout_plan_size() { return sizeof(DropPlan); }
 
 // tag null: tag_value.
 BLADES_API int blades_client_dropout(const void* x, void* y, const long* uids, const long* tag, long tag_value,

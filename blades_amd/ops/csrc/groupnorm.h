@@ -24,6 +24,7 @@
 // x 4 x 4 fp32 with a residual 32 and 54 (6.4, 5.2); two sweeps of 48 x 64 x 112 x 112 fp32 27 + 48 and 52 + 72 (5.9).
 #pragma once
 #include "common.h"
+#include "layers_abi.h"
 
 namespace groupnorm {
 

@@ -13,8 +13,9 @@
 // LDS and walks memory in order was slower, 95 against 73 us on the first: the index arithmetic of every vector and half the
 // waves cost more than the angles.)
 #include "common.h"
+#include "layers_abi.h"
 
-namespace {
+namespace rope {
 constexpr int TPB = 256;
 constexpr int MAX_PAIRS = 128;  // head dimension up to 256
 
@@ -129,7 +130,8 @@ inline int rows_of(long blocks, int rows) {
   while (per > 4 && blocks * ((rows + per - 1) / per) < 2048) per = (per + 1) / 2;
   return per;
 }
-}  // namespace
+}  // namespace rope
+using namespace rope;
 
 BLADES_API long blades_rope_plan_size() { return sizeof(RopePlan); }
 

@@ -468,3 +468,23 @@ def test_group_norm_plan_bounds_samples_times_chunks():
             taken += 1
             assert ws[1] // (8 * C) < (1 << 24) + 2048 + N  # (the means: at most N x G <= N x C entries)
     assert taken > 2000
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# builds that fit together
+def test_the_nodes_and_the_kernels_share_one_interface():
+    """Both libraries are made from one header, depend on it, and refuse a partner of another build."""
+    import ctypes
+    import importlib
+
+    from blades_amd.ops import build
+
+    abi = build.CSRC / "layers_abi.h"
+    for name in ("autograd.cpp", "groupnorm_fwd.hip", "groupnorm_bwd.hip", "dropout.hip", "rope.hip"):
+        assert abi in build._headers(build.CSRC / name), name
+    if not build.AUTOGRAD_LIB.exists():
+        pytest.skip("nodes are not built")
+    nodes = importlib.import_module("blades_amd.ops._autograd")
+    other = ctypes.CFUNCTYPE(ctypes.c_long)(lambda: 1)
+    with pytest.raises(RuntimeError, match="another build"):
+        nodes.entries([ctypes.cast(other, ctypes.c_void_p).value] * 9)
