@@ -29,20 +29,39 @@ ARCH = "gfx950"
 NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
-def _stale(target: Path, sources) -> bool:
+def _text(cmd) -> str:
+    """A command without the place it runs in: what a build depends on besides its sources."""
+    return " ".join(str(c) for c in cmd).replace(str(HERE), ".")
+
+
+def _stamp(target: Path) -> Path:
+    return HERE / "_build" / (target.name + ".cmd")
+
+
+def _stale(target: Path, sources, cmd=()) -> bool:
+    """Is the target missing, older than a source, or made by another command?"""
     if not target.exists():
         return True
     t = target.stat().st_mtime
-    return any(Path(s).stat().st_mtime > t for s in sources)
+    if any(Path(s).stat().st_mtime > t for s in sources):
+        return True
+    stamp = _stamp(target)
+    return not stamp.exists() or stamp.read_text() != _text(cmd)
+
+
+def _made(target: Path, cmd) -> None:
+    _stamp(target).parent.mkdir(exist_ok=True)
+    _stamp(target).write_text(_text(cmd))
 
 
 def build_host(force: bool = False, verbose: bool = False) -> Path:
     srcs = [CSRC / "host.cpp"]
-    if force or _stale(HOST_LIB, srcs):
-        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-o", str(HOST_LIB)] + [str(s) for s in srcs]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-o", str(HOST_LIB)] + [str(s) for s in srcs]
+    if force or _stale(HOST_LIB, srcs, cmd):
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)
+        _made(HOST_LIB, cmd)
     return HOST_LIB
 
 
@@ -68,48 +87,54 @@ def build_hip(force: bool = False, verbose: bool = False, jobs: int = 4) -> Path
     objdir.mkdir(exist_ok=True)
     procs = []
     objs = []
+
+    def done(s0, o0, cmd0, p0):
+        if p0.wait() != 0:
+            raise RuntimeError(f"hipcc failed on {s0}")
+        _made(o0, cmd0)
+
     for s in srcs:
         o = objdir / (s.stem + ".o")
         objs.append(o)
-        if force or _stale(o, [s] + _headers(s)):
-            cmd = [HIPCC, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-c", str(s), "-o", str(o),
-                   "-I", str(CSRC), "-Wno-unused-result"] + NO_PACKED_FP32
+        cmd = [HIPCC, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-c", str(s), "-o", str(o),
+               "-I", str(CSRC), "-Wno-unused-result"] + NO_PACKED_FP32
+        if force or _stale(o, [s] + _headers(s), cmd):
             if verbose:
                 print(" ".join(cmd), flush=True)
-            procs.append((s, subprocess.Popen(cmd)))
+            procs.append((s, o, cmd, subprocess.Popen(cmd)))
             if len(procs) >= jobs:
-                s0, p0 = procs.pop(0)
-                if p0.wait() != 0:
-                    raise RuntimeError(f"hipcc failed on {s0}")
-    for s0, p0 in procs:
-        if p0.wait() != 0:
-            raise RuntimeError(f"hipcc failed on {s0}")
-    if force or _stale(HIP_LIB, objs):
-        cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(HIP_LIB)] + [str(o) for o in objs]
+                done(*procs.pop(0))
+    for job in procs:
+        done(*job)
+    cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(HIP_LIB)] + [str(o) for o in objs]
+    if force or _stale(HIP_LIB, objs, cmd):
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)
+        _made(HIP_LIB, cmd)
     return HIP_LIB
 
 
 def build_autograd(force: bool = False, verbose: bool = False) -> Path:
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
     src = CSRC / "autograd.cpp"
-    if force or _stale(AUTOGRAD_LIB, [src] + _headers(src)):
-        import sysconfig
-
-        import torch
-        from torch.utils.cpp_extension import include_paths
-
-        lib = Path(torch.__file__).parent / "lib"
-        rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
-        inc = include_paths() + [f"{rocm}/include", sysconfig.get_paths()["include"]]
-        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-               "-DTORCH_EXTENSION_NAME=_autograd", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-        cmd += [a for i in inc for a in ("-isystem", i)] + [str(src), "-o", str(AUTOGRAD_LIB), f"-L{lib}", "-ltorch",
-                                                            "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip"]
+    lib = Path(torch.__file__).parent / "lib"
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    inc = include_paths() + [f"{rocm}/include", sysconfig.get_paths()["include"]]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           "-DTORCH_EXTENSION_NAME=_autograd", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    cmd += [a for i in inc for a in ("-isystem", i)] + [str(src), "-o", str(AUTOGRAD_LIB), f"-L{lib}", "-ltorch",
+                                                        "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip"]
+    made_of = cmd + ["#", torch.__version__]  # (the nodes are PyTorch's: another version's headers, another build)
+    if force or _stale(AUTOGRAD_LIB, [src] + _headers(src), made_of):
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.check_call(cmd)
+        _made(AUTOGRAD_LIB, made_of)
     return AUTOGRAD_LIB
 
 

@@ -488,3 +488,31 @@ def test_the_nodes_and_the_kernels_share_one_interface():
     other = ctypes.CFUNCTYPE(ctypes.c_long)(lambda: 1)
     with pytest.raises(RuntimeError, match="another build"):
         nodes.entries([ctypes.cast(other, ctypes.c_void_p).value] * 9)
+
+
+def test_objects_depend_on_their_command(tmp_path, monkeypatch):
+    """A changed flag, source or header makes a target stale; another folder does not."""
+    import os
+
+    from blades_amd.ops import build
+
+    monkeypatch.setattr(build, "HERE", tmp_path)
+    src, out = tmp_path / "a.hip", tmp_path / "a.o"
+    cmd = ["hipcc", "-O3", str(src), "-o", str(out)]
+    src.write_text("")
+    assert build._stale(out, [src], cmd)
+    out.write_text("")
+    assert build._stale(out, [src], cmd)  # made by nobody knows what
+    build._made(out, cmd)
+    assert not build._stale(out, [src], cmd)
+    assert build._stale(out, [src], cmd + ["-Xclang", "-packed-fp32-ops"])
+    os.utime(src, (out.stat().st_mtime + 5,) * 2)
+    assert build._stale(out, [src], cmd)
+    moved = tmp_path / "moved"
+    moved.mkdir()
+    (moved / "_build").mkdir()
+    (moved / "_build" / "a.o.cmd").write_text((tmp_path / "_build" / "a.o.cmd").read_text())
+    (moved / "a.hip").write_text("")
+    (moved / "a.o").write_text("")
+    monkeypatch.setattr(build, "HERE", moved)
+    assert not build._stale(moved / "a.o", [moved / "a.hip"], ["hipcc", "-O3", moved / "a.hip", "-o", moved / "a.o"])
