@@ -81,7 +81,7 @@ def hip_sources():
     return sorted(CSRC.glob("*.hip"))
 
 
-def build_hip(force: bool = False, verbose: bool = False, jobs: int = 4) -> Path:
+def build_hip(force: bool = False, verbose: bool = False, jobs: int = 8) -> Path:
     srcs = hip_sources()
     objdir = HERE / "_build"
     objdir.mkdir(exist_ok=True)
