@@ -1260,6 +1260,16 @@ class FusedFedSGD:
     def end_round(self):
         self.sink.planes_valid = False
 
+    def _logits(self, x):
+        """The template's forward pass.  Feature maps are channels last here: a model that asks for another layout
+        (``x.view(x.size(0), -1)`` on maps of several pixels) is declined, for the general executors to run."""
+        try:
+            return self.template(x)
+        except RuntimeError as e:
+            if "view size is not compatible" not in str(e):
+                raise
+            raise NotImplementedError(f"the model views its feature maps in another layout than channels last: {e}") from e
+
     def run(self, X: torch.Tensor, Y: torch.Tensor, block: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
         """X [Kc, B, ...], Y [Kc, B]; ``block`` = the chunk's rows of U (row stride
         preserved); returns per-client losses [Kc] (fp32, detached)."""
@@ -1275,7 +1285,7 @@ class FusedFedSGD:
 
         with fused_scope():
             # the input needs no gradient: first-layer backward skips its dgrad
-            logits = self.template(x)
+            logits = self._logits(x)
             return self._loss_backward(logits, Y, Kc, B)
 
     def _loss_backward(self, logits, Y, Kc, B):
@@ -1321,7 +1331,7 @@ class FusedFedSGD:
             from blades_amd.ops.activations import fused_scope
 
             with torch.enable_grad(), fused_scope():
-                logits = self.template(x)
+                logits = self._logits(x)
                 losses = self._loss_backward(logits, Y, Kc, B)
             missing = [k for k in self.sink.offsets if not self.sink._written.has(k)]
             if missing:
@@ -1347,7 +1357,7 @@ class FusedFedSGD:
         from blades_amd.ops.activations import fused_scope
 
         with fused_scope():
-            out = self.template(x).float().reshape(Kc, m, -1)
+            out = self._logits(x).float().reshape(Kc, m, -1)
         self.template.train()
         return out
 

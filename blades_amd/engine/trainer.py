@@ -487,6 +487,11 @@ class ClientEngine:
         self._graph_loss_pair = ent["loss_pair"]
         return ent["losses"]
 
+    def _decline_fused(self, e):
+        """The fused executor does not take this model after all: the general executors run it from here on."""
+        self.fused, self.fused_pc, self.fused_pc_error = None, False, str(e)
+        self._ensure_grouped()
+
     def _train_chunk_fedsgd(self, theta, rows, srows):
         self._local_step = 0
         if self._graphs_wanted():
@@ -502,12 +507,17 @@ class ClientEngine:
         rows_t = self._chunk_consts(rows)[0]
         contiguous = int(rows[-1] - rows[0]) == len(rows) - 1
         plain = self.momentum == 0.0 and not self._any_clip
+        losses = None
         if self.fused is not None:
             # per-client gradients land in the rows of U directly, pre-scaled
             block = self.U_row[int(rows[0]): int(rows[-1]) + 1] if contiguous else torch.empty(
                 len(rows), self.D, device=self.device)
             scale = (-self.lr * gscale) if plain else torch.ones_like(gscale)
-            losses = self.fused.run(X, Y, block, scale.float())
+            try:
+                losses = self.fused.run(X, Y, block, scale.float())
+            except NotImplementedError as e:
+                self._decline_fused(e)
+        if losses is not None:
             if plain:
                 if not contiguous:
                     self.U_row[rows_t, : self.D] = block
@@ -1017,7 +1027,8 @@ class ClientEngine:
             with _autocast(self.device, self.amp_dtype):
                 return functional_call(self.model, params, (x,)).float()
 
-        vf = self.fused.forward_only if self.fused is not None else vmap(fwd, in_dims=0, randomness="different")
+        general = vmap(fwd, in_dims=0, randomness="different")
+        vf = self.fused.forward_only if self.fused is not None else general
         by_len: Dict[int, List[int]] = {}
         for r, n in enumerate(st.lengths):
             by_len.setdefault(int(n), []).append(r)
@@ -1037,7 +1048,14 @@ class ClientEngine:
                     Y = st.y[idx.reshape(-1)].reshape(len(rr), m)
                     if tf is not None:
                         X = tf(X)
-                    logits = vf(X)
+                    try:
+                        logits = vf(X)
+                    except NotImplementedError as e:
+                        if vf is general:
+                            raise
+                        self._decline_fused(e)
+                        vf = general
+                        logits = vf(X)
                     acc += ops.ce_topk(logits.reshape(-1, logits.shape[-1]), Y.reshape(-1), ks)  # fused CE + top-k
                     count += Y.numel()
         if self.fused is not None:

@@ -516,3 +516,41 @@ def test_objects_depend_on_their_command(tmp_path, monkeypatch):
     (moved / "a.o").write_text("")
     monkeypatch.setattr(build, "HERE", moved)
     assert not build._stale(moved / "a.o", [moved / "a.hip"], ["hipcc", "-O3", moved / "a.hip", "-o", moved / "a.o"])
+
+
+def viewing(norm):
+    class Viewing(nn.Module):
+        """Flattens maps of several pixels with ``view``, which asks for channels first."""
+
+        def __init__(self):
+            super().__init__()
+            self.conv, self.norm, self.fc = nn.Conv2d(3, 8, 3, stride=4), norm(), nn.Linear(8 * 64, 10)
+
+        def forward(self, x):
+            x = nn.functional.silu(self.norm(self.conv(x)))
+            return self.fc(x.view(x.size(0), -1))
+
+    return Viewing
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("first", ["train", "evaluate"])
+@pytest.mark.parametrize("nb", [1, 2])
+@pytest.mark.parametrize("norm", [nn.Identity, lambda: nn.GroupNorm(2, 8)], ids=["none", "group"])
+def test_a_model_that_views_its_maps_channels_first(data_root, norm, nb, first):
+    """The fused executor, channels last throughout, hands it to the general ones."""
+    from tests.test_batch_independent_models import gpu_copy
+
+    a = build(data_root, viewing(norm), "vmap", nb=nb, lr=0.05)
+    g = gpu_copy(a, "auto")
+    assert g.engine.fused is not None
+    want = a.engine.evaluate(a.server.theta)
+    if first == "evaluate":
+        got = g.engine.evaluate(g.server.theta)
+        assert g.engine.fused is None and abs(got["ce_loss"] - want["ce_loss"]) < 1e-4
+    Ug, Ua = one_round_updates(g)[0].cpu(), one_round_updates(a)[0]
+    # two fp32 paths of under 100 operations in a chain, each off by under 16 half steps of its scale, over two steps
+    assert float(((Ug - Ua).norm(dim=1) / Ua.norm(dim=1)).max()) < 4e-4
+    assert "layout" in g.engine.fused_pc_error
+    got, want = g.engine.evaluate(g.server.theta), a.engine.evaluate(a.server.theta)
+    assert abs(got["ce_loss"] - want["ce_loss"]) < 1e-3
