@@ -84,12 +84,14 @@ __global__ __launch_bounds__(TPB) void rope_kernel(Freq f, Shape q, int per, con
     };
     fetch(r0);
     float sn[VEC / 2], cs[VEC / 2];
+    bool still[VEC / 2];  // pairs that pass through: as they are (a turn by 0 would let an infinity into its neighbour)
     if (turns) {
 #pragma unroll
       for (int j = 0; j < VEC / 2; ++j) {
         const int pair = l * (VEC / 2) + j, a = f.axis[pair];
         sn[j] = 0.f; cs[j] = 1.f;
-        if (a != 255) {
+        still[j] = a == 255;
+        if (!still[j]) {
           const long o = r * q.psr + n * q.A + a;
           const double p = q.pos_float ? (double)static_cast<const float*>(pos)[o] : (double)static_cast<const long*>(pos)[o];
           sincos_turns(p * f.turns[pair], sn[j], cs[j]);
@@ -105,8 +107,11 @@ __global__ __launch_bounds__(TPB) void rope_kernel(Freq f, Shape q, int per, con
 #pragma unroll
             for (int j = 0; j < VEC / 2; ++j) {
               const float a = to_f(w[u].e[2 * j]), b = to_f(w[u].e[2 * j + 1]);
-              from_f(fmaf(a, cs[j], -b * sn[j]), w[u].e[2 * j]);
-              from_f(fmaf(a, sn[j], b * cs[j]), w[u].e[2 * j + 1]);
+              T ta, tb;
+              from_f(fmaf(a, cs[j], -b * sn[j]), ta);
+              from_f(fmaf(a, sn[j], b * cs[j]), tb);
+              w[u].e[2 * j] = still[j] ? w[u].e[2 * j] : ta;
+              w[u].e[2 * j + 1] = still[j] ? w[u].e[2 * j + 1] : tb;
             }
           }
           store_out(y + (same ? (size_t)at[u] : yo + (size_t)(row + u) * q.D), w[u], q.through);

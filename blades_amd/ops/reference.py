@@ -495,6 +495,6 @@ def rope_axes(x, pos, axes, base: float = 10000.0, slots=None, inverse: bool = F
     rot = 2 * freq.numel()
     pf = part.to(acc)
     a, b = pf[..., 0:rot:2], pf[..., 1:rot:2]
-    y = torch.stack((a * cos - b * sin, a * sin + b * cos), dim=-1).flatten(-2)
-    y = torch.cat((y, pf[..., rot:]), dim=-1).to(x.dtype)
+    y = torch.stack((a * cos - b * sin, a * sin + b * cos), dim=-1).flatten(-2).to(x.dtype)
+    y = torch.cat((y, part[..., rot:]), dim=-1)
     return y if rest is None else torch.cat((y, rest), dim=2)

@@ -554,3 +554,40 @@ def test_a_model_that_views_its_maps_channels_first(data_root, norm, nb, first):
     assert "layout" in g.engine.fused_pc_error
     got, want = g.engine.evaluate(g.server.theta), a.engine.evaluate(a.server.theta)
     assert abs(got["ce_loss"] - want["ce_loss"]) < 1e-3
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# rotary positions
+def through(device, dt):
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(2, 3, 1, 2, 24, generator=g).to(dt)
+    x[..., 12::3] = float("inf")
+    x[..., 13::3] = float("nan")
+    x[..., 14::3] = -0.0
+    x[0, 0, 0, 0, 20:] = torch.tensor([torch.finfo(dt).tiny / 2, -torch.finfo(dt).tiny / 4, -0.0, -torch.finfo(dt).max])
+    x = x.to(device).requires_grad_(True)
+    pos = torch.arange(1, 4, device=device).unsqueeze(1)
+    y = ops.rope_axes(x, pos, (10,))
+    return x.detach(), y.detach(), torch.autograd.grad(y, x, x.detach())[0]
+
+
+def bits(t):
+    return t.contiguous().view(torch.int32 if t.element_size() == 4 else torch.int16)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+def test_the_rest_of_the_head_passes_through_cpu(dt):
+    x, y, dx = through("cpu", dt)
+    assert torch.equal(bits(y[..., 10:]), bits(x[..., 10:])) and bool(torch.isfinite(y[..., :10]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+def test_the_rest_of_the_head_passes_through(dev, dt):
+    """Bit for bit, both ways: an infinity does not reach its neighbour, a zero keeps its sign."""
+    x, y, dx = through(dev, dt)
+    assert torch.equal(bits(y[..., 10:]), bits(x[..., 10:])) and torch.equal(bits(dx[..., 10:]), bits(x[..., 10:]))
+    assert bool(torch.isfinite(y[..., :10]).all())
+    z = x.clone()
+    ops._h().rope_axes(z, torch.arange(1, 4, device=dev).unsqueeze(1), (10,), out=z)
+    assert torch.equal(bits(z), bits(y))
