@@ -591,3 +591,30 @@ def test_the_rest_of_the_head_passes_through(dev, dt):
     z = x.clone()
     ops._h().rope_axes(z, torch.arange(1, 4, device=dev).unsqueeze(1), (10,), out=z)
     assert torch.equal(bits(z), bits(y))
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# what a model does with an output
+@pytest.mark.gpu
+@pytest.mark.parametrize("spatial", [(), (5,), (4, 3), (1, 1), (2, 3, 4)])
+def test_outputs_may_be_changed_in_place(dev, spatial):
+    """As those of any operator: an in-place activation or residual add behind the layer, in the engine's module too."""
+    from blades_amd.engine.fused import GradSink, PCGroupNorm
+
+    sink = GradSink()
+    sink.Kc = 1
+    m = PCGroupNorm(nn.GroupNorm(2, 8, affine=False), sink)
+    x = torch.randn(3, 8, *spatial, device=dev)
+    for f in (lambda t: ops.group_norm(t, 2), m, lambda t: ops.client_dropout(t, torch.zeros((), dtype=torch.int64, device=dev),
+                                                                           1, 1, 0, 0.5)):
+        a, b = (x.clone().requires_grad_(True) for _ in range(2))
+        y = f(a)
+        y.mul_(3).add_(a)
+        z = f(b) * 3 + b
+        assert torch.equal(y, z)
+        gy = torch.randn_like(x)
+        assert torch.equal(torch.autograd.grad(y, a, gy)[0], torch.autograd.grad(z, b, gy)[0])
+    t = torch.randn(2, 5, 3, 2, 8, device=dev, requires_grad=True)
+    y = ops.rope_axes(t, torch.arange(5, device=dev).unsqueeze(1), (4,), slots=2)
+    y.mul_(2)
+    y.sum().backward()
