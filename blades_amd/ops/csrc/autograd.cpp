@@ -44,7 +44,17 @@ hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.
 
 int dtype_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? 0 : t.scalar_type() == at::kBFloat16 ? 1 : 2; }
 
-template <typename T = void> T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
+// Gradients and what hooks unpack can be tensors without memory (wrapper subclasses, batches of gradients under a transform):
+// those raise, in front of any launch.
+void check_memory(const Tensor& t) {
+  TORCH_CHECK(t.has_storage() && (t.numel() == 0 || t.data_ptr() != nullptr), "the batch-independent layers take tensors with "
+              "memory of their own; their gradients are not batched");
+}
+template <typename T = void> T* ptr(const Tensor& t) {
+  if (!t.defined()) return nullptr;
+  check_memory(t);
+  return static_cast<T*>(t.data_ptr());
+}
 
 // Saved tensors can pass through hooks (moved to the host and back, say): the kernels rely on these.
 void check_saved(const char* name, bool ok) {
@@ -150,6 +160,7 @@ variable_list GroupNormBackward::apply(variable_list&& grads) {
   variable_list out(4);
   Tensor gy = std::move(grads[0]);
   if (!gy.defined()) return out;
+  check_memory(gy);
   const bool nx = task_should_compute_output(0), nw = has_w && task_should_compute_output(1),
              nb = has_b && task_should_compute_output(2), nr = has_res && task_should_compute_output(3);
   {
@@ -257,6 +268,7 @@ struct ClientDropoutBackward : Node {
   variable_list apply(variable_list&& grads) override {
     variable_list out(1);
     if (!grads[0].defined()) return out;
+    check_memory(grads[0]);
     {
       at::NoGradGuard no_grad;
       out[0] = drop(grads[0], uids.unpack(shared_from_this()), tag.unpack(shared_from_this()), tag_value, p);
@@ -338,7 +350,7 @@ Tensor turn(const Tensor& t, const Tensor& pos, const Rope& r, int inverse) {
   const Tensor p = pos.contiguous();
   const int w = x.scalar_type() == at::kFloat ? 4 : 8;
   auto step = [&] { return x.stride(0) | x.stride(1) | x.stride(2) | x.stride(-2); };
-  const auto at_ = [&] { return reinterpret_cast<uintptr_t>(x.data_ptr()); };
+  const auto at_ = [&] { return reinterpret_cast<uintptr_t>(ptr(x)); };
   int vec = w;
   if (at_() % 16 || step() % w || x.size(-1) % w) {
     if (step() % 2 || at_() % (2 * x.element_size())) x = x.clone(at::MemoryFormat::Contiguous);
@@ -358,6 +370,7 @@ struct RopeBackward : Node {
   variable_list apply(variable_list&& grads) override {
     variable_list out(1);
     if (!grads[0].defined()) return out;
+    check_memory(grads[0]);
     {
       at::NoGradGuard no_grad;
       out[0] = turn(grads[0], pos.unpack(shared_from_this()), r, 1);

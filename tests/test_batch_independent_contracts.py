@@ -618,3 +618,20 @@ def test_outputs_may_be_changed_in_place(dev, spatial):
     y = ops.rope_axes(t, torch.arange(5, device=dev).unsqueeze(1), (4,), slots=2)
     y.mul_(2)
     y.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", LAYERS)
+def test_gradients_without_memory_are_refused(dev, name):
+    """A wrapper subclass as gradient, a batch of gradients: raised, nothing launched on their addresses."""
+    f, args = layers(dev)[name]
+    leaves = [a.detach().clone(memory_format=torch.preserve_format).requires_grad_(True) for a in args]
+    y = f(leaves)
+    gy = torch.ones_like(y)
+    want = torch.autograd.grad(y, leaves, gy, retain_graph=True)
+    with pytest.raises(RuntimeError, match="memory of their own"):
+        torch.autograd.grad(y, leaves, Doubled(gy), retain_graph=True)
+    with pytest.raises(RuntimeError, match="memory of their own"):
+        torch.autograd.grad(y, leaves, torch.stack([gy, gy]), is_grads_batched=True, retain_graph=True)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, gy), want))
