@@ -50,6 +50,11 @@ void check_memory(const Tensor& t) {
   TORCH_CHECK(t.has_storage() && (t.numel() == 0 || t.data_ptr() != nullptr), "the batch-independent layers take tensors with "
               "memory of their own; their gradients are not batched");
 }
+void check_gradient(const Tensor& t) {
+  check_memory(t);
+  // (a tangent on a gradient asks for a second derivative)
+  TORCH_CHECK(!t._fw_grad(0).defined(), "the batch-independent layers are differentiable once: their gradients take no tangent");
+}
 template <typename T = void> T* ptr(const Tensor& t) {
   if (!t.defined()) return nullptr;
   check_memory(t);
@@ -160,7 +165,7 @@ variable_list GroupNormBackward::apply(variable_list&& grads) {
   variable_list out(4);
   Tensor gy = std::move(grads[0]);
   if (!gy.defined()) return out;
-  check_memory(gy);
+  check_gradient(gy);
   const bool nx = task_should_compute_output(0), nw = has_w && task_should_compute_output(1),
              nb = has_b && task_should_compute_output(2), nr = has_res && task_should_compute_output(3);
   {
@@ -268,7 +273,7 @@ struct ClientDropoutBackward : Node {
   variable_list apply(variable_list&& grads) override {
     variable_list out(1);
     if (!grads[0].defined()) return out;
-    check_memory(grads[0]);
+    check_gradient(grads[0]);
     {
       at::NoGradGuard no_grad;
       out[0] = drop(grads[0], uids.unpack(shared_from_this()), tag.unpack(shared_from_this()), tag_value, p);
@@ -370,7 +375,7 @@ struct RopeBackward : Node {
   variable_list apply(variable_list&& grads) override {
     variable_list out(1);
     if (!grads[0].defined()) return out;
-    check_memory(grads[0]);
+    check_gradient(grads[0]);
     {
       at::NoGradGuard no_grad;
       out[0] = turn(grads[0], pos.unpack(shared_from_this()), r, 1);

@@ -635,3 +635,17 @@ def test_gradients_without_memory_are_refused(dev, name):
         torch.autograd.grad(y, leaves, torch.stack([gy, gy]), is_grads_batched=True, retain_graph=True)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, gy), want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", LAYERS)
+def test_a_gradients_tangent_is_refused(dev, name):
+    """Forward over reverse with the tangent behind the layer: a second derivative, which raises as the others do."""
+    f, args = layers(dev)[name]
+    leaves = [a.detach().clone(memory_format=torch.preserve_format).requires_grad_(True) for a in args]
+    y = f(leaves)
+    gy = torch.ones_like(y)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(y, leaves, forward_ad.make_dual(gy, gy), retain_graph=True)
+        torch.autograd.grad(y, leaves, gy)
