@@ -948,7 +948,7 @@ class PCBatchNorm2d(nn.Module):
 
 
 class _PCGroupNormFn(torch.autograd.Function):
-    """Group norm with fused residual add and activation (ops/csrc/groupnorm.hip); each client's affine gradients go,
+    """Group norm with fused residual add and activation (ops/csrc/groupnorm_{fwd,bwd}.hip); each client's affine gradients go,
     scaled, into its update row.  Statistics are a sample's own, so clients matter to the affine pair alone.  Shapes the
     kernel does not take, and the CPU, run the oracle, the backward pass through autograd on it."""
 

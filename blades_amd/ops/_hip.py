@@ -1785,7 +1785,7 @@ def ce_topk(logits, labels, ks):
 
 
 # ---------------------------------------------------------------------------
-# layers whose result for a sample does not depend on who shares the batch: group norm (ops/csrc/groupnorm.hip),
+# layers whose result for a sample does not depend on who shares the batch: group norm (ops/csrc/groupnorm_{fwd,bwd}.hip),
 # client-keyed dropout without a stored mask (dropout.hip), rotary positions with several axes (rope.hip)
 _DT_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACT_CODE = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}

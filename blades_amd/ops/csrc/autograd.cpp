@@ -337,8 +337,8 @@ std::shared_ptr<std::vector<char>> rope_plan(const Tensor& x, const Tensor& pos,
   for (auto& k : kept)
     if (k.first == key) return k.second;
   auto plan = std::make_shared<std::vector<char>>(lib.rope_plan_size());
-  const int rc = lib.rope_plan(reinterpret_cast<rope::RopePlan*>(plan->data()), pf, psr, R, N, S, H, D, x.stride(0), x.stride(1), five ? x.stride(2) : 0,
-                               x.stride(-2), r.slots, r.axes.data(), (int)r.axes.size(), r.base, dt, vec);
+  const int rc = lib.rope_plan(reinterpret_cast<rope::RopePlan*>(plan->data()), pf, psr, R, N, S, H, D, x.stride(0),
+                               x.stride(1), five ? x.stride(2) : 0, x.stride(-2), r.slots, r.axes.data(), (int)r.axes.size(), r.base, dt, vec);
   if (rc != 0) throw py::value_error("rope_axes: rejected (rc=" + std::to_string(rc) + ")");
   if (kept.size() >= 16) kept.erase(kept.begin());
   kept.emplace_back(std::move(key), plan);

@@ -19,9 +19,11 @@
 // forward + backward 380 us in pieces of 96 MB, 319 in 180 MB, 292 at once).  All sums are fp32 in a fixed order (double
 // where many partial sums meet): bitwise reproducible.
 //
-// Bound by memory.  Measured (MI355X; copies run at 5.0 - 5.4 TB/s beyond the last-level cache, at 8 within it): 2048 x 64 x
-// 32 x 32 fp32 forward 198 us (5.4 TB/s), backward 320 (5.0); 2048 x 128 x 16 x 16 bf16 SiLU 47 and 80 (5.7, 5.0); 2048 x 512
-// x 4 x 4 fp32 with a residual 32 and 54 (6.4, 5.2); two sweeps of 48 x 64 x 112 x 112 fp32 27 + 48 and 52 + 72 (5.9).
+// Bound by memory.  Kernel times on average over training passes (MI355X; copies run at 5.0 - 5.4 TB/s beyond the last-level
+// cache, at 8 within it): 2048 x 64 x 32 x 32 fp32 forward 196 us (5.5 TB/s), backward 332 (4.9); 2048 x 128 x 16 x 16 bf16 SiLU
+// 50 and 91 (5.4, 4.4); 2048 x 512 x 4 x 4 fp32 with a residual 33 and 56 (6.2, 4.9); two sweeps of 48 x 64 x 112 x 112 fp32
+// GELU 28 + 49 and 53 + 74.  fp16 is slower than bf16 (2048 x 128 x 16 x 16: 70 and 187 us against 46 and 77): its conversions
+// to 32 bits stay in registers, and the backward kernel's no longer fit.
 #pragma once
 #include "common.h"
 #include "layers_abi.h"
@@ -227,10 +229,11 @@ inline bool make_plan(Plan& pl, long N, long P, int C, int G, int esize, int vec
   q.per_client = per_client;
   q.first = 0;
   q.back = 0;
-  // Outputs of up to 256 MB, the last-level cache, are stored past it: 2048 x 128 x 16 x 16 bf16 (128 MB) forward 47 us
-  // against 51, backward 79 against 94 (with a producer and a consumer of equal size around them 134 against 142, 173
-  // against 183); 2048 x 512 x 4 x 4 fp32 (64 MB) 120 against 104 a pass alone, 61 against 64 forward in such a chain.
-  // Beyond it that costs: 2048 x 64 x 32 x 32 fp32 (512 MB) 538 us a pass against 554, in a chain 548 against 573 forward.
+  // Outputs of up to 256 MB, the last-level cache, are stored past it.  Kernel times on average, stored past it against through
+  // it: repeated alone / in a row of three with a product of equal size in front and behind.
+  //   2048 x 128 x 16 x 16 bf16 (128 MB)  forward 53 : 64 / 147 : 151   backward 104 : 115 / 206 : 207
+  //   2048 x 512 x 4 x 4 fp32 (64 MB)     forward 31 : 36 /  87 :  85   backward  55 :  60 / 104 : 107
+  //   2048 x 64 x 32 x 32 fp32 (512 MB)   forward 212 : 193 / 577 : 547 backward 321 : 328 / 666 : 663   (hence the limit)
   q.through = N * P * C * esize <= (256L << 20);
   // Slabs: as few as give workgroups of at most 256 threads x `maxr` vectors, but with pixel rows of at least a cache
   // line (128 bytes).  Narrower ones (down to 64 bytes) only where a sample would not fit a workgroup otherwise, and down

@@ -8,10 +8,10 @@
 // others copied (v).  A thread owns 16 bytes of the head dimension of one token: while its first rows are on their way, its two
 // (four) angles are computed, once for all its rows (slots and heads): the turns (position times frequency, reduced to an
 // eighth) in 64 bits so that far positions keep theirs, sine and cosine by their Taylor polynomials in 32 bits.
-// Memory-bound: every byte is read and written once.  Measured: 2048 x 64 x 3 x 2 x 64 fp32 74 us (5.4 TB/s), 8 x 3136 x 3 x
-// 6 x 64 bf16 with per-sample positions 23 (5.0; 19 without the angles).  (A workgroup that shares its tokens' angles through
-// LDS and walks memory in order was slower, 95 against 73 us on the first: the index arithmetic of every vector and half the
-// waves cost more than the angles.)
+// Memory-bound: every byte is read and written once.  Kernel times on average over training passes: 2048 x 64 x 3 x 2 x 64
+// fp32 74 us (5.5 TB/s), 8 x 3136 x 3 x 6 x 64 bf16 with per-sample positions 23 (5.0; 19 without the angles).  (A workgroup that
+// shares its tokens' angles through LDS and walks memory in order was slower, 95 against 73 us on the first: the index arithmetic
+// of every vector and half the waves cost more than the angles.)
 #include "common.h"
 #include "layers_abi.h"
 
@@ -156,8 +156,10 @@ BLADES_API int blades_rope_plan(RopePlan* p, int pos_float, long psr, long R, lo
     }
   }
   for (; pair < MAX_PAIRS; ++pair) { p->f.turns[pair] = 0.0; p->f.axis[pair] = 255; }
-  // Outputs of up to 256 MB, the last-level cache, are stored past it: 2048 x 64 x 3 x 2 x 64 fp32 62 us against 78 (with a
-  // producer and a consumer of equal size around it 201 against 212), 8 x 3136 x 3 x 6 x 64 bf16 23 against 27 (59, 61).
+  // Outputs of up to 256 MB, the last-level cache, are stored past it.  Kernel times on average, stored past it against through
+  // it: forward passes over one input / in a row of three with a product of equal size in front and behind.
+  //   2048 x 64 x 3 x 2 x 64 fp32    62 : 79 / 203 : 217
+  //   8 x 3136 x 3 x 6 x 64 bf16     23 : 24 /  59 :  59
   const long bytes = R * N * S * H * D * (dtype == 0 ? 4 : 2);
   p->q = Shape{R, N, sr, sn, ss, sh, S, H, D, A, rot, S, psr, pos_float, 0, bytes <= (256L << 20)};
   p->dtype = dtype; p->vec = vec;

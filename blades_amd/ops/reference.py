@@ -425,7 +425,7 @@ def shuffle_keys(uids, epochs, lens, nmax: int, seed: int):
 
 
 def group_norm(x, groups: int, weight=None, bias=None, eps: float = 1e-5, act: str = "none", residual=None):
-    """Oracle of ops/csrc/groupnorm.hip: ``act(group_norm(x) * weight + bias + residual)`` for ``x [N, C, *]``;
+    """Oracle of ops/csrc/groupnorm_fwd.hip: ``act(group_norm(x) * weight + bias + residual)`` for ``x [N, C, *]``;
     ``weight`` / ``bias`` ``[C]``, or ``[K, C]`` for K clients of N / K consecutive samples each.  32-bit arithmetic
     (64 for 64-bit inputs), rounded once.  Differentiable (plain torch ops)."""
     acc = torch.float64 if x.dtype == torch.float64 else torch.float32
