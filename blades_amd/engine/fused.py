@@ -882,11 +882,12 @@ class PCMaxPool2d(nn.Module):
     def extra_repr(self):
         return f"kernel_size={self.k}, stride={self.s}, padding={self.p}, relu_folded={self.relu}"
 
-    def forward(self, x):
+    def forward(self, x, relu: bool = False):
+        relu = relu or self.relu
         if x.is_cuda and x.dim() == 4 and _hipmod().maxpool_supported(x, self.k, self.s, self.p, self.dilation,
                                                                       self.ceil_mode):
-            return _MaxPoolFn.apply(x, self.k, self.s, self.p, self.relu)
-        if self.relu:
+            return _MaxPoolFn.apply(x, self.k, self.s, self.p, relu)
+        if relu:
             x = F.relu(x)
         return F.max_pool2d(x, self.k, self.s, self.p, self.dilation, self.ceil_mode)
 
@@ -1032,16 +1033,22 @@ class PCGroupNorm(nn.Module):
 
 
 class PCSequential(nn.Sequential):
-    """A Sequential that runs a group norm and the activation directly behind it as one kernel.  Both stay modules of their
-    own, so a model that calls, slices or walks the children itself gets what they compute."""
+    """A Sequential that runs a group norm and the activation directly behind it, or a ReLU and the max-pool behind that, as one
+    kernel.  All stay modules of their own, so a model that calls, slices or walks the children itself gets what they compute."""
 
     def forward(self, x):
         kids = list(self._modules.values())
         i = 0
         while i < len(kids):
-            fold = i + 1 < len(kids) and type(kids[i]) is PCGroupNorm and _behind_group_norm(kids[i + 1]) == kids[i].act
-            x = kids[i](x, folded=True) if fold else kids[i](x)
-            i += 2 if fold else 1
+            m, behind = kids[i], kids[i + 1] if i + 1 < len(kids) else None
+            i += 2
+            if type(m) is PCGroupNorm and behind is not None and _behind_group_norm(behind) == m.act:
+                x = m(x, folded=True)
+            elif type(m) is PCActivation and m.kind == "relu" and type(behind) is PCMaxPool2d:
+                x = behind(x, relu=True)
+            else:
+                x = m(x)
+                i -= 1
         return x
 
 
@@ -1160,22 +1167,23 @@ def build_template(model: nn.Module, sink: GradSink) -> nn.Module:
     tmpl = copy.deepcopy(model, memo)
 
     def swap(mod):
-        if isinstance(mod, nn.Sequential):
-            # ReLU directly in front of a max-pool: folded into the pooling kernel (FashionCNN, the CCT tokenizers)
-            kids = list(mod.named_children())
-            for (n0, c0), (n1, c1) in zip(kids, kids[1:]):
-                if type(c0) is nn.ReLU and isinstance(c1, nn.MaxPool2d):
-                    setattr(mod, n0, nn.Identity())
-                    setattr(mod, n1, PCMaxPool2d(c1, relu=True))
         if type(mod) is nn.Sequential:
-            # an activation directly behind a group norm (a module that stands in several places is listed at each of them
-            # here): PCSequential runs both in one kernel
+            # an activation directly behind a group norm, a ReLU directly in front of a max-pool (a module that stands in
+            # several places is listed at each of them here): PCSequential runs both in one kernel
             kids = list(mod._modules.items())
             for (n0, c0), (n1, c1) in zip(kids, kids[1:]):
                 act = _behind_group_norm(c1) if type(c0) is nn.GroupNorm else None
                 if act is not None:
                     setattr(mod, n0, PCGroupNorm(c0, sink, act))
+                if act is not None or (type(c0) is nn.ReLU and isinstance(c1, nn.MaxPool2d)):
                     mod.__class__ = PCSequential
+        elif isinstance(mod, nn.Sequential):
+            # ReLU directly in front of a max-pool, in a Sequential with a forward of its own: folded for good
+            kids = list(mod.named_children())
+            for (n0, c0), (n1, c1) in zip(kids, kids[1:]):
+                if type(c0) is nn.ReLU and isinstance(c1, nn.MaxPool2d):
+                    setattr(mod, n0, nn.Identity())
+                    setattr(mod, n1, PCMaxPool2d(c1, relu=True))
         for name, child in list(mod._modules.items()):  # (a module that stands in several places: at each of them)
             if child is None:
                 continue

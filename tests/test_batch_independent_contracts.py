@@ -271,6 +271,34 @@ class Tapped(nn.Module):
         return torch.cat([a, b, c, d, self.body(x)], 1)
 
 
+class TappedPool(nn.Module):
+    """The same with a pool behind the activation."""
+
+    def __init__(self):
+        super().__init__()
+        self.body = nn.Sequential(nn.Conv2d(3, 8, 1), nn.GroupNorm(2, 8), nn.ReLU(), nn.MaxPool2d(2), nn.Conv2d(8, 8, 1),
+                                  nn.ReLU(), nn.MaxPool2d(2, 1))
+
+    def forward(self, x):
+        h = self.body[1](self.body[0](x))
+        r = self.body[2](h)
+        p = self.body[3](r - 0.5)  # the pool alone
+        q = self.body[5](self.body[4](p))
+        return [h, r, p, q, self.body[6](q - 0.5), self.body[4:6](p), self.body(x)]
+
+
+def test_a_models_own_use_of_a_pool():
+    from blades_amd.engine.fused import GradSink, build_template
+
+    net, sink = TappedPool(), GradSink()
+    sink.Kc = 2
+    tmpl = build_template(net, sink)
+    x = torch.randn(4, 3, 6, 6)
+    with torch.no_grad():
+        for a, b in zip(tmpl(x), net(x)):
+            torch.testing.assert_close(a, b, rtol=1e-5, atol=1e-5)
+
+
 def test_a_models_own_use_of_a_sequentials_children():
     from blades_amd.engine.fused import GradSink, build_template
 
