@@ -38,13 +38,15 @@ def _stamp(target: Path) -> Path:
     return HERE / "_build" / (target.name + ".cmd")
 
 
-def _stale(target: Path, sources, cmd=()) -> bool:
-    """Is the target missing, older than a source, or made by another command?"""
+def _stale(target: Path, sources, cmd=None) -> bool:
+    """Is the target missing, older than a source, or (where one is given) made by another command?"""
     if not target.exists():
         return True
     t = target.stat().st_mtime
     if any(Path(s).stat().st_mtime > t for s in sources):
         return True
+    if cmd is None:
+        return False
     stamp = _stamp(target)
     return not stamp.exists() or stamp.read_text() != _text(cmd)
 
@@ -52,6 +54,12 @@ def _stale(target: Path, sources, cmd=()) -> bool:
 def _made(target: Path, cmd) -> None:
     _stamp(target).parent.mkdir(exist_ok=True)
     _stamp(target).write_text(_text(cmd))
+
+
+def host_lib() -> Path:
+    """What is built, for loading: made here only where it is missing or older than its source (an installed package has no
+    record of the command)."""
+    return build_host() if _stale(HOST_LIB, [CSRC / "host.cpp"]) else HOST_LIB
 
 
 def build_host(force: bool = False, verbose: bool = False) -> Path:

@@ -13,7 +13,7 @@ LINKAGES = {"single": 0, "average": 1, "complete": 2}
 def lib():
     global _lib
     if _lib is None:
-        path = _build.build_host()
+        path = _build.host_lib()
         _lib = ctypes.CDLL(str(path))
         _lib.blades_agglomerative2.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p]
         _lib.blades_kmeans.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_uint64,

@@ -677,3 +677,24 @@ def test_a_gradients_tangent_is_refused(dev, name):
         with pytest.raises(RuntimeError, match="differentiable once"):
             torch.autograd.grad(y, leaves, forward_ad.make_dual(gy, gy), retain_graph=True)
         torch.autograd.grad(y, leaves, gy)
+
+
+def test_an_installed_host_library_is_loaded_not_built(tmp_path, monkeypatch):
+    """A package without a record of how it was built (a wheel) loads its library as it is."""
+    import os
+    import subprocess
+
+    from blades_amd.ops import build
+
+    lib, src = tmp_path / "libblades_host.so", tmp_path / "csrc" / "host.cpp"
+    src.parent.mkdir()
+    src.write_text("")
+    lib.write_text("")
+    for name, value in (("HERE", tmp_path), ("CSRC", src.parent), ("HOST_LIB", lib)):
+        monkeypatch.setattr(build, name, value)
+    monkeypatch.setattr(subprocess, "check_call", lambda cmd: built.append(cmd))
+    built = []
+    os.utime(lib, (src.stat().st_mtime + 5,) * 2)
+    assert build.host_lib() == lib and not built
+    os.utime(src, (lib.stat().st_mtime + 5,) * 2)
+    assert build.host_lib() == lib and len(built) == 1
