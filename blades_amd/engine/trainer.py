@@ -489,6 +489,8 @@ class ClientEngine:
 
     def _decline_fused(self, e):
         """The fused executor does not take this model after all: the general executors run it from here on."""
+        if self.device.type == "cuda":
+            torch.cuda.synchronize(self.device)  # (its buffers go with it, and other streams' kernels may still read them)
         self.fused, self.fused_pc, self.fused_pc_error = None, False, str(e)
         self._ensure_grouped()
 
